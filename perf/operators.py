@@ -263,7 +263,7 @@ def _codes(kv, x):
     big = x.abs().max(-1, keepdim=True)
     top = 127 if kv == "q8" else 7
     if kv == "q8":
-        d = big.values / 127
+        d = big.values / torch.full_like(big.values, 127.0)  # (by a number it is a product with 1 / 127)
     else:
         d = x.gather(-1, big.indices) / -8
     d = d.clamp(-65504, 65504).half()
