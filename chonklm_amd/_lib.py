@@ -20,6 +20,10 @@ CHONK_ELOST = -6
 CHONK_ENOMEM = -7
 KV_F16 = 0
 KV_F32 = 1
+KV_Q8 = 2
+KV_Q4 = 3
+F32 = 0
+F16 = 1
 
 STATUS_NAMES = {
     CHONK_EINVAL: "EINVAL",
@@ -114,6 +118,65 @@ class SynthConfigC(C.Structure):
     ]
 
 
+class KvCacheC(C.Structure):
+    _fields_ = [
+        ("kv_type", C.c_int32),
+        ("kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("n_pages", C.c_int32),
+        ("pages", C.c_void_p),
+        ("n_seqs", C.c_int32),
+        ("max_pages", C.c_int32),
+        ("table", C.c_void_p),
+        ("fault", C.c_void_p),
+        ("device", C.c_int32),
+    ]
+
+
+class KvRowsC(C.Structure):
+    _fields_ = [("n", C.c_int32), ("seq", C.c_void_p), ("pos", C.c_void_p)]
+
+
+class KvAppendArgsC(C.Structure):
+    _fields_ = [
+        ("type", C.c_int32),
+        ("heads", C.c_int32),
+        ("q", C.c_void_p),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("q_out", C.c_void_p),
+        ("q_stride", C.c_int64),
+        ("k_stride", C.c_int64),
+        ("v_stride", C.c_int64),
+        ("q_out_stride", C.c_int64),
+        ("q_norm", C.c_void_p),
+        ("k_norm", C.c_void_p),
+        ("eps", C.c_double),
+        ("rope", C.c_void_p),
+        ("rope_dim", C.c_int32),
+        ("rope_positions", C.c_int32),
+        ("interleaved", C.c_int32),
+    ]
+
+
+class KvAttendArgsC(C.Structure):
+    _fields_ = [
+        ("type", C.c_int32),
+        ("heads", C.c_int32),
+        ("n", C.c_int32),
+        ("seq", C.c_void_p),
+        ("lengths", C.c_void_p),
+        ("q", C.c_void_p),
+        ("out", C.c_void_p),
+        ("q_stride", C.c_int64),
+        ("out_stride", C.c_int64),
+        ("scale", C.c_float),
+        ("window", C.c_int32),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+    ]
+
+
 P = C.c_void_p
 I32P = C.POINTER(C.c_int32)
 TOKEN_CALLBACK = C.CFUNCTYPE(C.c_int32, C.c_void_p, C.c_int32, C.c_int32)
@@ -152,6 +215,11 @@ SIGNATURES = [
     ("chonk_batch_step", C.c_int, [P, I32P, I32P, C.c_size_t, I32P]),
     ("chonk_batch_position", C.c_int, [P, C.c_int32, I32P]),
     ("chonk_batch_read_logits", C.c_int, [P, C.c_int32, F32P, C.c_size_t]),
+    ("chonk_kv_page_bytes", C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),
+    ("chonk_kv_append", C.c_int, [C.POINTER(KvCacheC), C.POINTER(KvRowsC), C.POINTER(KvAppendArgsC), P]),
+    ("chonk_kv_read", C.c_int, [C.POINTER(KvCacheC), C.POINTER(KvRowsC), C.c_int32, P, P, C.c_int64, C.c_int64, P]),
+    ("chonk_kv_attend_workspace", C.c_int64, [C.POINTER(KvCacheC), C.c_int32, C.c_int32]),
+    ("chonk_kv_attend", C.c_int, [C.POINTER(KvCacheC), C.POINTER(KvAttendArgsC), P]),
     ("chonk_engine_time_kernels", C.c_int, [P, I32P, C.c_int32, C.c_int32, C.POINTER(C.c_double)]),
     ("chonk_engine_bench_kernel", C.c_int,
      [P, C.c_int32, C.c_int32, C.POINTER(C.c_double), C.c_char_p, C.c_size_t, C.POINTER(C.c_uint64)]),

@@ -38,6 +38,7 @@
 #include "../host/gguf.h"
 #include "../host/synth.h"
 #include "chonk.h"
+#include "errors.h"
 #include "kernels.h"
 #include "prefill.h"
 
@@ -58,21 +59,10 @@ bool multi_off() {
 static __device__ __align__(256) uint8_t scratch[kNoAllocScratchBytes];
 
 namespace chonk {
-namespace {
 
 thread_local std::string g_last_error;
 
-struct Error : std::runtime_error {
-  int code;
-  Error(int c, const std::string& m) : std::runtime_error(m), code(c) {}
-};
-
-#define HIP_OK(expr)                                                                               \
-  do {                                                                                             \
-    hipError_t e_ = (expr);                                                                        \
-    if (e_ != hipSuccess)                                                                          \
-      throw Error(CHONK_EHIP, std::string("HIP error ") + hipGetErrorString(e_) + " at " #expr);  \
-  } while (0)
+namespace {
 
 // ---- repacking GGUF blocks into stripes -------------------------------------------
 
@@ -657,20 +647,6 @@ int api(chonk_engine* e, F&& f) {
     g_last_error = x.what();
     if (e) e->err = x.what();
     return CHONK_EINVAL;
-  }
-}
-
-template <typename F>
-int api_free(F&& f) {
-  try {
-    f();
-    return CHONK_OK;
-  } catch (const Error& x) {
-    g_last_error = x.what();
-    return x.code;
-  } catch (const std::exception& x) {
-    g_last_error = x.what();
-    return CHONK_EIO;
   }
 }
 

@@ -1,0 +1,930 @@
+// The quantised, paged K/V cache for gfx950: new rows normalised, rotated and
+// quantised into their pages (k_kv_append), values read back (k_kv_read), and
+// attention of one new token a row over the pages, split over the length and
+// joined (k_kv_attend, k_kv_join). The C entry points are at the end.
+//
+// A page holds 64 positions; per kv head K codes | K scales | V codes | V scales.
+// Codes come in units of 32 positions x 32 dims, in the order in which lane
+// n = 16 g + i of a wave feeds the 16x16x32 matrix product:
+//   scores   S[position][head] = K Q^T: A row i = position 16 t + i, k = dims 8 g + e
+//   output   O[dim][head]      = V^T P^T: A row i = dim 16 h + i, k = positions
+//            4 g + (e & 3) + 16 (e >> 2)
+// The scores' result leaves lane (g, head) with positions 4 g + r of both tiles
+// t = 0, 1: exactly the eight positions that the second product's B operand
+// wants there, so the probabilities never leave their lane.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <string>
+
+#include "chonk.h"
+#include "errors.h"
+#include "kernel_common.h"
+#include "part_sum.h"
+#include "paged_kv.h"
+
+namespace chonk {
+namespace {
+
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f4_t mfma(h8_t a, h8_t b, f4_t c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ void fault(const KvCache& c, int bit) {
+  if (c.fault) atomicOr(c.fault, bit);
+}
+
+// The page of (seq, pos), or -1 (and the fault noted) where there is none.
+__device__ __forceinline__ int page_of(const KvCache& c, int seq, int pos, bool note) {
+  const int bad = seq >= c.n_seqs ? KVF_SEQ : pos < 0 || pos / kKvPage >= c.max_pages ? KVF_POS : 0;
+  if (bad) {
+    if (note) fault(c, bad);
+    return -1;
+  }
+  const int page = c.table[(size_t)seq * c.max_pages + pos / kKvPage];
+  if (page < 0 || page >= c.n_pages) {
+    if (note) fault(c, KVF_PAGE);
+    return -1;
+  }
+  return page;
+}
+
+// Place of position p (0..31 of its half) in the order of the scales and of
+// the V operand: lane group 4 bits up, its eight positions below.
+__device__ __forceinline__ int place_of(int p) { return ((p & 15) >> 2) * 8 + (p & 3) + 4 * (p >> 4); }
+
+// ---- writing ----------------------------------------------------------------------
+
+// Codes and scale of eight lanes' 32 values, four consecutive dims a lane. A
+// scale is the fp16 nearest to the exact one, and the codes count in units of
+// that fp16 number, so a code is off by at most half a unit of what is stored.
+template <int KV>
+__device__ __forceinline__ uint32_t quantise(const float (&y)[4], int (&c)[4]) {
+  constexpr float kTop = KV == CHONK_KV_Q8 ? 127.f : 7.f, kLow = KV == CHONK_KV_Q8 ? -127.f : -8.f;
+  float m = 0.f;
+  int bad = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (fabsf(y[i]) > fabsf(m)) m = y[i];
+    bad |= !(fabsf(y[i]) <= 3.402823466e38f);
+  }
+#pragma unroll
+  for (int x = 1; x < 8; x *= 2) {
+    const float o = __shfl_xor(m, x);
+    bad |= __shfl_xor(bad, x);
+    // (of equal magnitudes the lower dim's: every lane must find the same one)
+    if (fabsf(o) > fabsf(m) || (fabsf(o) == fabsf(m) && (threadIdx.x & x))) m = o;
+  }
+  float d = KV == CHONK_KV_Q8 ? __fdiv_rn(fabsf(m), 127.f) : m * -0.125f;
+  d = fminf(fmaxf(d, -65504.f), 65504.f);
+  const _Float16 h = (_Float16)d;
+  const float dh = (float)h;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    c[i] = bad || dh == 0.f ? 0 : (int)fminf(fmaxf(rintf(__fdiv_rn(y[i], dh)), kLow), kTop);
+  return bad ? 0x7e00u : (uint32_t)__builtin_bit_cast(unsigned short, h);
+}
+
+// Four consecutive values of K (or V) at dims d0 .. d0 + 3 of position j of the
+// page into the head's part at `base`. The eight lanes of a block come together.
+template <int KV, bool IS_V>
+__device__ __forceinline__ void put4(uint8_t* base, int hd, int j, int d0, const float (&y)[4], bool ok) {
+  const int nb = hd / 32, b = d0 / 32, u = j / 32, p = j & 31, i0 = d0 & 31;
+  const int unit = u * nb + b;
+  if constexpr (KV == CHONK_KV_F16) {
+    _Float16* o = (_Float16*)base + (size_t)unit * 1024;
+    h4_t v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (_Float16)y[i];
+    if (!ok) return;
+    if constexpr (!IS_V) {
+      *(h4_t*)(o + (p >> 4) * 512 + ((i0 >> 3) * 16 + (p & 15)) * 8 + (i0 & 7)) = v;
+    } else {
+      const int pl = place_of(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        o[(i0 >> 4) * 512 + ((pl >> 3) * 16 + (i0 & 15) + i) * 8 + (pl & 7)] = v[i];
+    }
+  } else {
+    int c[4];
+    const uint32_t d = quantise<KV>(y, c);
+    const int pl = place_of(p);
+    uint16_t* sc = (uint16_t*)(base + kv_code_bytes(KV, hd));
+    if (ok && i0 == 0) sc[unit * 32 + pl] = (uint16_t)d;
+    if constexpr (KV == CHONK_KV_Q8) {
+      uint8_t* o = base + (size_t)unit * 1024;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] += 128;
+      if (!ok) return;
+      if constexpr (!IS_V) {
+        *(uint32_t*)(o + ((i0 >> 3) * 16 + (p & 15)) * 16 + (p >> 4) * 8 + (i0 & 7)) =
+            (uint32_t)(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          o[((pl >> 3) * 16 + (i0 & 15) + i) * 16 + (i0 >> 4) * 8 + (pl & 7)] = (uint8_t)c[i];
+      }
+    } else {
+      uint8_t* o = base + (size_t)unit * 512;
+      // the lane with the other nibbles: dims + 4 (K), dims + 16 (V)
+      constexpr int X = IS_V ? 4 : 1;
+      int n[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c[i] += 8;
+        n[i] = c[i] | __shfl_xor(c[i], X) << 4;
+      }
+      if (!ok || (threadIdx.x & X)) return;
+      if constexpr (!IS_V) {
+        *(uint32_t*)(o + ((i0 >> 3) * 16 + (p & 15)) * 8 + (p >> 4) * 4) =
+            (uint32_t)(n[0] | n[1] << 8 | n[2] << 16 | n[3] << 24);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[((pl >> 3) * 16 + (i0 & 15) + i) * 8 + (pl & 7)] = (uint8_t)n[i];
+      }
+    }
+  }
+}
+
+// Four consecutive elements of a row.
+template <bool F16>
+__device__ __forceinline__ void row4(const PartSum& P, const _Float16* p16, int64_t ld, int r, int col, float (&v)[4]) {
+  if constexpr (F16) {
+    const _Float16* p = p16 + r * ld + col;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = (float)p[i];
+  } else {
+    const int j[4] = {col, col + 1, col + 2, col + 3};
+    part_gather<4>(P, r, j, v);
+  }
+}
+
+// One wave per (row, head): q heads, then kv heads (K and V). Lane t holds dims
+// 4 t .. 4 t + 3, so a block of 32 is eight lanes. Every product and sum after
+// the norm's is rounded by itself (no fused multiply-add) and the norm's sum of squares is taken in 64
+// bits: the codes do not depend on which path (prompt rows or single tokens)
+// wrote them.
+template <int KV, bool F16>
+__global__ __launch_bounds__(kWg) void k_kv_append(KvAppendArgs a) {
+#pragma clang fp contract(off)
+  __shared__ float xs[4][256];
+  const int r = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int hh = blockIdx.y * 4 + wave, qh = (F16 ? a.q16 != nullptr : a.q.p != nullptr) ? a.heads : 0;
+  if (hh >= qh + a.c.kv_heads) return;
+  const int seq = a.at.seq ? a.at.seq[r] : a.at.seq0, pos = a.at.pos ? a.at.pos[r] : a.at.p0 + r;
+  if (seq < 0) return;
+  const int hd = a.c.hd, d0 = 4 * lane;
+  const bool ok = d0 < hd, is_k = hh >= qh;
+  const int kv = hh - qh;
+  const int page = page_of(a.c, seq, pos, lane == 0);
+  if (page < 0) return;
+  if (a.rope && pos >= a.rope_n) {
+    if (lane == 0) fault(a.c, KVF_POS);
+    return;
+  }
+  float y[4] = {0.f, 0.f, 0.f, 0.f};
+  if (ok) row4<F16>(is_k ? a.k : a.q, is_k ? a.k16 : a.q16, is_k ? a.k_ld : a.q_ld, r, (is_k ? kv : hh) * hd + d0, y);
+  const float* w = is_k ? a.kn_w : a.qn_w;
+  if (w) {
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss += (double)y[i] * (double)y[i];
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) ss += __shfl_xor(ss, x);
+    const float inv = (float)(1.0 / sqrt(ss / hd + a.eps));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = ok ? y[i] * inv * w[d0 + i] : 0.f;
+  }
+  if (a.rope) {
+    float* x = xs[wave];
+    if (ok) *(float4*)(x + d0) = make_float4(y[0], y[1], y[2], y[3]);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const int half = a.rope_dim / 2;
+    const float2* cs = a.rope + (size_t)pos * half;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = d0 + i;
+      if (d >= a.rope_dim) continue;
+      const int pair = a.interleaved ? d >> 1 : d < half ? d : d - half;
+      const bool second = a.interleaved ? (d & 1) != 0 : d >= half;
+      const float2 t = cs[pair];
+      const float u = x[a.interleaved ? 2 * pair : pair], v = x[a.interleaved ? 2 * pair + 1 : pair + half];
+      y[i] = second ? u * t.y + v * t.x : u * t.x - v * t.y;
+    }
+  }
+  if (!is_k) {
+    if (!ok) return;
+    const int64_t o = r * a.qo_ld + hh * hd + d0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (F16)
+        ((_Float16*)a.q_out)[o + i] = (_Float16)y[i];
+      else
+        ((float*)a.q_out)[o + i] = y[i];
+    }
+    return;
+  }
+  const int part = kv_part_bytes(KV, hd), j = pos & (kKvPage - 1);
+  uint8_t* base = a.c.pages + ((size_t)page * a.c.kv_heads + kv) * 2 * part;
+  put4<KV, false>(base, hd, j, d0, y, ok);
+  if (ok)
+    row4<F16>(a.v, a.v16, a.v_ld, r, kv * hd + d0, y);
+  else
+    y[0] = y[1] = y[2] = y[3] = 0.f;
+  put4<KV, true>(base + part, hd, j, d0, y, ok);
+}
+
+// ---- reading back -----------------------------------------------------------------
+
+// One thread per (row, kv head, eight dims).
+template <int KV, bool F16>
+__global__ __launch_bounds__(kWg) void k_kv_read(KvReadArgs a) {
+  const int hd = a.c.hd, runs = hd / 8;
+  const int64_t id = (int64_t)blockIdx.x * kWg + threadIdx.x;
+  const int64_t rk = id / runs;
+  const int d0 = (int)(id % runs) * 8, kv = (int)(rk % a.c.kv_heads);
+  const int64_t r = rk / a.c.kv_heads;
+  if (r >= a.rows) return;
+  const int seq = a.at.seq ? a.at.seq[r] : a.at.seq0, pos = a.at.pos ? a.at.pos[r] : a.at.p0 + (int)r;
+  if (seq < 0) return;
+  const int page = page_of(a.c, seq, pos, d0 == 0);
+  if (page < 0) return;
+  const int part = kv_part_bytes(KV, hd), j = pos & (kKvPage - 1), p = j & 31, pl = place_of(p);
+  const int unit = (j / 32) * (hd / 32) + d0 / 32, i0 = d0 & 31;
+  const uint8_t* base = a.c.pages + ((size_t)page * a.c.kv_heads + kv) * 2 * part;
+  const int64_t o = r * a.row_ld + kv * a.head_ld + d0;
+#pragma unroll
+  for (int is_v = 0; is_v < 2; ++is_v) {
+    void* out = is_v ? a.v : a.k;
+    if (!out) continue;
+    const uint8_t* src = base + is_v * part;
+    float x[8];
+    if constexpr (KV == CHONK_KV_F16) {
+      const _Float16* h = (const _Float16*)src + (size_t)unit * 1024;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        x[i] = is_v ? (float)h[(i0 >> 4) * 512 + ((pl >> 3) * 16 + (i0 & 15) + i) * 8 + (pl & 7)]
+                    : (float)h[(p >> 4) * 512 + ((i0 >> 3) * 16 + (p & 15)) * 8 + i];
+    } else {
+      const float d = h2f(((const uint16_t*)(src + kv_code_bytes(KV, hd)))[unit * 32 + pl]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        int c;
+        if constexpr (KV == CHONK_KV_Q8) {
+          const uint8_t* q = src + (size_t)unit * 1024;
+          c = (is_v ? q[((pl >> 3) * 16 + (i0 & 15) + i) * 16 + (i0 >> 4) * 8 + (pl & 7)]
+                    : q[((i0 >> 3) * 16 + (p & 15)) * 16 + (p >> 4) * 8 + i]) - 128;
+        } else {
+          const uint8_t* q = src + (size_t)unit * 512;
+          const int byte = is_v ? q[((pl >> 3) * 16 + (i0 & 15) + i) * 8 + (pl & 7)]
+                                : q[((i0 >> 3) * 16 + (p & 15)) * 8 + (p >> 4) * 4 + (i & 3)];
+          c = ((is_v ? i0 >> 4 : i >> 2) ? byte >> 4 : byte & 15) - 8;
+        }
+        x[i] = (float)c * d;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (F16)
+        ((_Float16*)out)[o + i] = (_Float16)x[i];
+      else
+        ((float*)out)[o + i] = x[i];
+    }
+  }
+}
+
+// ---- attention --------------------------------------------------------------------
+
+// Eight codes as exact halves. Bytes come through v_perm beside 0x64 (1024 + c
+// is exact in fp16) and the bias goes in one packed subtraction, so the halves'
+// order is (0, 2, 1, 3, 4, 6, 5, 7): both products take their k in that order.
+__device__ __forceinline__ h2_t bias2(uint32_t v, float b) {
+  const _Float16 h = (_Float16)b;
+  return __builtin_bit_cast(h2_t, v) - h2_t{h, h};
+}
+__device__ __forceinline__ h8_t codes8(uint32_t w0, uint32_t w1) {
+  constexpr uint32_t kE = 0x64646464u;
+  const h2_t a = bias2(__builtin_amdgcn_perm(kE, w0, 0x04020400u), 1152.f);
+  const h2_t b = bias2(__builtin_amdgcn_perm(kE, w0, 0x04030401u), 1152.f);
+  const h2_t c = bias2(__builtin_amdgcn_perm(kE, w1, 0x04020400u), 1152.f);
+  const h2_t d = bias2(__builtin_amdgcn_perm(kE, w1, 0x04030401u), 1152.f);
+  return h8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// The low (H = 0) or high nibbles of the words' bytes; the high ones as 16 times the code.
+template <int H>
+__device__ __forceinline__ h4_t nibbles4(uint32_t w) {
+  constexpr uint32_t kM = H ? 0x00f000f0u : 0x000f000fu;
+  const float b = H ? 1152.f : 1032.f;
+  const h2_t x = bias2((w & kM) | 0x64006400u, b), y = bias2(((w >> 8) & kM) | 0x64006400u, b);
+  return h4_t{x[0], x[1], y[0], y[1]};
+}
+__device__ __forceinline__ h8_t join(h4_t a, h4_t b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+template <int KV>
+constexpr int kOrder(int e) {  // element e of an operand's k: which of the eight
+  if (KV == CHONK_KV_F16) return e;
+  constexpr int o[8] = {0, 2, 1, 3, 4, 6, 5, 7};
+  return o[e];
+}
+
+// One workgroup per (row, kv head, up to 16 of its q heads, segment of the
+// row's pages); its four waves take the pages in turn, each with its own running
+// maximum, sum and output, and meet in LDS at the end.
+template <int KV, int NB>
+__global__ __launch_bounds__(kWg) void k_kv_attend(KvAttendArgs a) {
+  constexpr int HD = 32 * NB;
+  constexpr int CODES = kv_code_bytes(KV, HD), PART = kv_part_bytes(KV, HD);
+  constexpr int UNIT = CODES / (2 * NB);
+  extern __shared__ __align__(16) float sm[];  // [wave][head][HD] | [wave][head][m, l]
+  const int G = a.heads / a.c.kv_heads, hgs = (G + 15) / 16;
+  int id = blockIdx.x;
+  const int seg = id % a.nseg;
+  id /= a.nseg;
+  const int hg = id % hgs;
+  id /= hgs;
+  const int kv = id % a.c.kv_heads, r = id / a.c.kv_heads;
+  const int h0 = kv * G + hg * 16, nh = min(16, G - hg * 16);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, col = lane & 15;
+
+  const int seq = ld_scalar(a.seq + r);
+  if (seq < 0) return;  // (the join leaves the row alone too)
+  int len = ld_scalar(a.len + r) + a.len_add;
+  bool bad = false;
+  if (len > 0 && (seq >= a.c.n_seqs || len > a.c.max_pages * kKvPage)) {
+    if (tid == 0) fault(a.c, seq >= a.c.n_seqs ? KVF_SEQ : KVF_POS);
+    bad = true;
+    len = 0;
+  }
+  const int first = a.window > 0 ? max(0, len - a.window) : 0;
+  const int pg0 = first / kKvPage, pg1 = (max(len, 0) + kKvPage - 1) / kKvPage;
+  const int per = (pg1 - pg0 + a.nseg - 1) / a.nseg;
+  const int from = pg0 + seg * per, to = min(from + per, pg1);
+
+  // q: this lane's head at dims 32 b + 8 g + e, scaled by a power of two so that the
+  // head's largest lies in [2^13, 2^14) and split into two halves of 11 bits each
+  h8_t qh[NB], ql[NB];
+  float mul;  // score of S in powers of two
+  {
+    float x[NB][8];
+    const int h = h0 + min(col, nh - 1);
+    const int64_t o = r * a.q_ld + (int64_t)h * HD + 8 * g;
+    float top = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int64_t at = o + 32 * b + kOrder<KV>(e);
+        x[b][e] = a.f16 ? (float)((const _Float16*)a.q)[at] : ((const float*)a.q)[at];
+        top = fmaxf(top, fabsf(x[b][e]));
+      }
+    float t0, t1;
+    swap16(top, t0, t1);
+    top = fmaxf(t0, t1);
+    swap32(top, t0, t1);
+    top = fmaxf(t0, t1);
+    const int sh = top > 0.f ? min(13 - ilogbf(top), 100) : 0;
+    mul = ldexpf(a.scale * 1.44269504f, -sh);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        // (the high nibbles are 16 times their code)
+        const float y = ldexpf(x[b][e], sh - (KV == CHONK_KV_Q4 && e >= 4 ? 4 : 0));
+        qh[b][e] = (_Float16)y;
+        ql[b][e] = (_Float16)(y - (float)qh[b][e]);
+      }
+  }
+
+  // m is the reference of the exponents: the running maximum mx less an offset
+  // that keeps weight * V scale within fp16 and its bits above fp16's denormals
+  float mx = -1e30f, m = -1e30f, l = 0.f, dtop = 0.f, off = KV == CHONK_KV_F16 ? 14.f : 0.f;
+  f4_t acc[2 * NB];
+#pragma unroll
+  for (int i = 0; i < 2 * NB; ++i) acc[i] = f4_t{0.f, 0.f, 0.f, 0.f};
+
+  for (int pg = from + wave; pg < to; pg += 4) {
+    const int page = ld_scalar(a.c.table + (size_t)seq * a.c.max_pages + pg);
+    if (page < 0 || page >= a.c.n_pages) {
+      if (lane == 0) fault(a.c, KVF_PAGE);
+      l = __builtin_nanf("");
+      continue;
+    }
+    const uint8_t* kb = a.c.pages + ((size_t)page * a.c.kv_heads + kv) * 2 * PART;
+    const uint8_t* vb = kb + PART;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int j0 = pg * kKvPage + 32 * u;
+      if (j0 >= len || j0 + 32 <= first) continue;
+      float s[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] = 0.f;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const uint8_t* unit = kb + (u * NB + b) * UNIT;
+        h8_t k0, k1;
+        if constexpr (KV == CHONK_KV_F16) {
+          k0 = __builtin_bit_cast(h8_t, ldg4(unit + lane * 16));
+          k1 = __builtin_bit_cast(h8_t, ldg4(unit + 1024 + lane * 16));
+        } else if constexpr (KV == CHONK_KV_Q8) {
+          const uint4 w = ldg4(unit + lane * 16);
+          k0 = codes8(w.x, w.y);
+          k1 = codes8(w.z, w.w);
+        } else {
+          const uint2 w = ldg2(unit + lane * 8);
+          k0 = join(nibbles4<0>(w.x), nibbles4<1>(w.x));
+          k1 = join(nibbles4<0>(w.y), nibbles4<1>(w.y));
+        }
+        const f4_t z = f4_t{0.f, 0.f, 0.f, 0.f};
+        const f4_t s0 = mfma(k0, ql[b], mfma(k0, qh[b], z));
+        const f4_t s1 = mfma(k1, ql[b], mfma(k1, qh[b], z));
+        if constexpr (KV == CHONK_KV_F16) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[e] += s0[e];
+            s[4 + e] += s1[e];
+          }
+        } else {
+          const h8_t d = __builtin_bit_cast(h8_t, ldg4(kb + CODES + (u * NB + b) * 64 + g * 16));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[e] = fmaf((float)d[e], s0[e], s[e]);
+            s[4 + e] = fmaf((float)d[4 + e], s1[e], s[4 + e]);
+          }
+        }
+      }
+      float top = -1e30f;
+      bool out[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = j0 + 4 * g + (e & 3) + 16 * (e >> 2);
+        out[e] = j < first || j >= len;
+        s[e] = out[e] ? -INFINITY : s[e] * mul;
+        top = fmaxf(top, s[e]);
+      }
+      float t0, t1;
+      swap16(top, t0, t1);
+      top = fmaxf(t0, t1);
+      swap32(top, t0, t1);
+      top = fmaxf(t0, t1);
+      h8_t dv[NB];
+      if constexpr (KV != CHONK_KV_F16) {
+        // the largest scale so far bounds weight * scale
+        float dm = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          dv[b] = __builtin_bit_cast(h8_t, ldg4(vb + CODES + (u * NB + b) * 64 + g * 16));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dm = fmaxf(dm, out[e] ? 0.f : fabsf((float)dv[b][e]));
+        }
+        swap16(dm, t0, t1);
+        dm = fmaxf(t0, t1);
+        swap32(dm, t0, t1);
+        dm = fminf(fmaxf(t0, t1), 65504.f);
+        if (dm > dtop) {
+          dtop = dm;
+          off = (float)(13 - ilogbf(dtop));  // weight * scale < 2^14
+        }
+      }
+      mx = fmaxf(mx, top);
+      const float ref = mx - off;
+      if (__ballot(ref != m)) {
+        const float f = exp2f(m - ref);
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) acc[i] *= f;
+        m = ref;
+      }
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = out[e] ? 0.f : exp2f(s[e] - m);
+        l += p[e];
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        h8_t ph, pl;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int k = kOrder<KV>(e);
+          float w = p[k];
+          if constexpr (KV != CHONK_KV_F16) w = out[k] ? 0.f : w * (float)dv[b][k];
+          ph[e] = (_Float16)w;
+          pl[e] = (_Float16)(w - (float)ph[e]);
+        }
+        const uint8_t* unit = vb + (u * NB + b) * UNIT;
+        h8_t v0, v1;
+        if constexpr (KV == CHONK_KV_F16) {
+          v0 = __builtin_bit_cast(h8_t, ldg4(unit + lane * 16));
+          v1 = __builtin_bit_cast(h8_t, ldg4(unit + 1024 + lane * 16));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {  // (what lies in unseen places may be anything)
+            v0[e] = out[e] ? (_Float16)0 : v0[e];
+            v1[e] = out[e] ? (_Float16)0 : v1[e];
+          }
+        } else if constexpr (KV == CHONK_KV_Q8) {
+          const uint4 w = ldg4(unit + lane * 16);
+          v0 = codes8(w.x, w.y);
+          v1 = codes8(w.z, w.w);
+        } else {
+          const uint2 w = ldg2(unit + lane * 8);
+          v0 = join(nibbles4<0>(w.x), nibbles4<0>(w.y));
+          v1 = join(nibbles4<1>(w.x), nibbles4<1>(w.y));
+        }
+        acc[2 * b] = mfma(v0, pl, mfma(v0, ph, acc[2 * b]));
+        acc[2 * b + 1] = mfma(v1, pl, mfma(v1, ph, acc[2 * b + 1]));
+      }
+    }
+  }
+  {
+    float t0, t1;
+    swap16(l, t0, t1);
+    l = t0 + t1;
+    swap32(l, t0, t1);
+    l = t0 + t1;
+  }
+  if (bad) l = __builtin_nanf("");
+  // the waves' rows meet in LDS
+  float* ml = sm + 4 * nh * HD;
+  if (col < nh) {
+    float* o = sm + (wave * nh + col) * HD;
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i) {
+      // (the V tiles from high nibbles are 16 times their codes)
+      const float f = KV == CHONK_KV_Q4 && (i & 1) ? 0.0625f : 1.f;
+      *(float4*)(o + 16 * i + 4 * g) = make_float4(acc[i][0] * f, acc[i][1] * f, acc[i][2] * f, acc[i][3] * f);
+    }
+    if (g == 0) {
+      ml[(wave * nh + col) * 2] = m;
+      ml[(wave * nh + col) * 2 + 1] = l;
+    }
+  }
+  __syncthreads();
+  for (int x = tid; x < nh * HD; x += kWg) {
+    const int h = x / HD, d = x % HD;
+    float M = -1e30f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[(w * nh + h) * 2]);
+    float L = 0.f, O = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = exp2f(ml[(w * nh + h) * 2] - M);
+      L += f * ml[(w * nh + h) * 2 + 1];
+      O += f * sm[(w * nh + h) * HD + d];
+    }
+    if (a.nseg > 1) {
+      float* p = a.part + (((int64_t)r * a.heads + h0 + h) * a.nseg + seg) * (HD + 2);
+      p[d] = O;
+      if (d == 0) {
+        p[HD] = M;
+        p[HD + 1] = L;
+      }
+    } else {
+      const float y = L == 0.f ? 0.f : O / L;
+      const int64_t o = r * a.o_ld + (int64_t)(h0 + h) * HD + d;
+      if (a.f16)
+        ((_Float16*)a.out)[o] = (_Float16)y;
+      else
+        ((float*)a.out)[o] = y;
+    }
+  }
+}
+
+// Joins a (row, head)'s segments, in their order.
+__global__ __launch_bounds__(kWg) void k_kv_join(KvAttendArgs a) {
+  const int h = blockIdx.x, r = blockIdx.y, hd = a.c.hd, d = threadIdx.x;
+  if (d >= hd || a.seq[r] < 0) return;
+  const float* p = a.part + ((int64_t)r * a.heads + h) * a.nseg * (hd + 2);
+  float M = -1e30f;
+  for (int s = 0; s < a.nseg; ++s) M = fmaxf(M, p[s * (hd + 2) + hd]);
+  float L = 0.f, O = 0.f;
+  for (int s = 0; s < a.nseg; ++s) {
+    const float f = exp2f(p[s * (hd + 2) + hd] - M);
+    L += f * p[s * (hd + 2) + hd + 1];
+    O += f * p[s * (hd + 2) + d];
+  }
+  const float y = L == 0.f ? 0.f : O / L;
+  const int64_t o = r * a.o_ld + (int64_t)h * hd + d;
+  if (a.f16)
+    ((_Float16*)a.out)[o] = (_Float16)y;
+  else
+    ((float*)a.out)[o] = y;
+}
+
+constexpr int kWantWgs = 1024;
+
+int attend_segments(const KvCache& c, int rows, int heads) {
+  const int64_t n = (int64_t)rows * c.kv_heads * ((heads / c.kv_heads + 15) / 16);
+  return (int)std::max<int64_t>(1, std::min<int64_t>((c.max_pages + 3) / 4, kWantWgs / n));
+}
+
+}  // namespace
+
+hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t s) {
+  const int nh = ((a.f16 ? a.q16 != nullptr : a.q.p != nullptr) ? a.heads : 0) + a.c.kv_heads;
+  const dim3 grid(a.rows, (nh + 3) / 4);
+#define CHONK_KV_CASE(T)                                                                \
+  case T:                                                                               \
+    if (a.f16)                                                                          \
+      hipLaunchKernelGGL((k_kv_append<T, true>), grid, dim3(kWg), 0, s, a);             \
+    else                                                                                \
+      hipLaunchKernelGGL((k_kv_append<T, false>), grid, dim3(kWg), 0, s, a);            \
+    return hipGetLastError();
+  switch (a.c.type) {
+    CHONK_KV_CASE(CHONK_KV_F16)
+    CHONK_KV_CASE(CHONK_KV_Q8)
+    CHONK_KV_CASE(CHONK_KV_Q4)
+    default: return hipErrorInvalidValue;
+  }
+#undef CHONK_KV_CASE
+}
+
+hipError_t launch_kv_read(const KvReadArgs& a, hipStream_t s) {
+  const int64_t n = (int64_t)a.rows * a.c.kv_heads * (a.c.hd / 8);
+  const dim3 grid((uint32_t)((n + kWg - 1) / kWg));
+#define CHONK_KV_CASE(T)                                                                \
+  case T:                                                                               \
+    if (a.f16)                                                                          \
+      hipLaunchKernelGGL((k_kv_read<T, true>), grid, dim3(kWg), 0, s, a);               \
+    else                                                                                \
+      hipLaunchKernelGGL((k_kv_read<T, false>), grid, dim3(kWg), 0, s, a);              \
+    return hipGetLastError();
+  switch (a.c.type) {
+    CHONK_KV_CASE(CHONK_KV_F16)
+    CHONK_KV_CASE(CHONK_KV_Q8)
+    CHONK_KV_CASE(CHONK_KV_Q4)
+    default: return hipErrorInvalidValue;
+  }
+#undef CHONK_KV_CASE
+}
+
+int64_t kv_attend_floats(const KvCache& c, int rows, int heads) {
+  const int nseg = attend_segments(c, rows, heads);
+  return nseg > 1 ? (int64_t)rows * heads * nseg * (c.hd + 2) : 0;
+}
+
+hipError_t launch_kv_attend(const KvAttendArgs& a0, hipStream_t s) {
+  KvAttendArgs a = a0;
+  const int G = a.heads / a.c.kv_heads, hgs = (G + 15) / 16, nh = std::min(G, 16);
+  a.nseg = attend_segments(a.c, a.rows, a.heads);
+  if (a.nseg > 1 && !a.part) return hipErrorInvalidValue;
+  const dim3 grid((uint32_t)((int64_t)a.rows * a.c.kv_heads * hgs * a.nseg));
+  const size_t sh = (size_t)4 * nh * (a.c.hd + 2) * 4;
+#define CHONK_KV_CASE(T, B)                                                                              \
+  if (a.c.type == T && a.c.hd == 32 * B) {                                                               \
+    if (sh > 65536) {                                                                                    \
+      const hipError_t e = hipFuncSetAttribute((const void*)k_kv_attend<T, B>,                           \
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)sh);     \
+      if (e != hipSuccess) return e;                                                                     \
+    }                                                                                                    \
+    hipLaunchKernelGGL((k_kv_attend<T, B>), grid, dim3(kWg), sh, s, a);                                  \
+  } else
+  CHONK_KV_CASE(CHONK_KV_F16, 1)
+  CHONK_KV_CASE(CHONK_KV_F16, 2)
+  CHONK_KV_CASE(CHONK_KV_F16, 4)
+  CHONK_KV_CASE(CHONK_KV_F16, 8)
+  CHONK_KV_CASE(CHONK_KV_Q8, 1)
+  CHONK_KV_CASE(CHONK_KV_Q8, 2)
+  CHONK_KV_CASE(CHONK_KV_Q8, 4)
+  CHONK_KV_CASE(CHONK_KV_Q8, 8)
+  CHONK_KV_CASE(CHONK_KV_Q4, 1)
+  CHONK_KV_CASE(CHONK_KV_Q4, 2)
+  CHONK_KV_CASE(CHONK_KV_Q4, 4)
+  CHONK_KV_CASE(CHONK_KV_Q4, 8)
+  return hipErrorInvalidValue;
+#undef CHONK_KV_CASE
+  if (a.nseg > 1) hipLaunchKernelGGL(k_kv_join, dim3(a.heads, a.rows), dim3(kWg), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace chonk
+
+// ---- C entry points -----------------------------------------------------------------
+
+namespace chonk {
+namespace {
+
+std::string no(const char* what, long long v) { return std::string(what) + " " + std::to_string(v); }
+
+void check_format(int32_t kv_type, int32_t kv_heads, int32_t head_dim) {
+  if (!kv_type_ok(kv_type)) throw Error(CHONK_EINVAL, no("paged K/V cache: unsupported kv type", kv_type));
+  if (kv_heads <= 0 || kv_heads > 4096) throw Error(CHONK_EINVAL, no("paged K/V cache: bad kv head count", kv_heads));
+  if (!kv_hd_ok(head_dim))
+    throw Error(CHONK_EINVAL, no("paged K/V cache: head_dim must be 32, 64, 128 or 256, not", head_dim));
+}
+
+KvCache checked(const chonk_kv_cache* c) {
+  if (!c) throw Error(CHONK_EINVAL, "null argument");
+  check_format(c->kv_type, c->kv_heads, c->head_dim);
+  if (c->n_pages <= 0 || c->n_seqs <= 0 || c->max_pages <= 0 || c->max_pages > (1 << 24) || !c->pages || !c->table)
+    throw Error(CHONK_EINVAL, "paged K/V cache: empty pool or table");
+  if ((uintptr_t)c->pages % 16) throw Error(CHONK_EINVAL, "paged K/V cache: pages must be 16-byte aligned");
+  KvCache k{};
+  k.pages = (uint8_t*)c->pages;
+  k.table = c->table;
+  k.fault = c->fault;
+  k.type = c->kv_type;
+  k.kv_heads = c->kv_heads;
+  k.hd = c->head_dim;
+  k.n_pages = c->n_pages;
+  k.n_seqs = c->n_seqs;
+  k.max_pages = c->max_pages;
+  return k;
+}
+
+void check_heads(int32_t heads, int32_t kv_heads) {
+  if (heads <= 0 || heads > 65536 || heads % kv_heads)
+    throw Error(CHONK_EINVAL, no("paged K/V cache: query heads must be a multiple of the kv heads, not", heads));
+}
+// A launch holds fewer than 2^32 threads.
+void check_grid(int64_t wgs) {
+  if (wgs >= (1 << 24)) throw Error(CHONK_EINVAL, "paged K/V cache: too many rows and heads for one call");
+}
+void check_rows(int32_t rows) {
+  if (rows < 0 || rows > (1 << 22)) throw Error(CHONK_EINVAL, no("paged K/V cache: bad row count", rows));
+}
+void check_act(int32_t type) {
+  if (type != CHONK_F32 && type != CHONK_F16) throw Error(CHONK_EINVAL, no("paged K/V cache: bad element type", type));
+}
+// Rows must not overlap (a row of a result) or run backwards.
+void check_stride(const char* what, int64_t ld, int64_t least) {
+  if (ld < least) throw Error(CHONK_EINVAL, std::string("paged K/V cache: ") + what + " rows are closer than their width");
+}
+
+// The cache's device for the length of a call.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    HIP_OK(hipGetDevice(&was_));
+    if (device != was_) HIP_OK(hipSetDevice(device));
+    now_ = device;
+  }
+  ~OnDevice() {
+    if (now_ != was_) (void)hipSetDevice(was_);
+  }
+
+ private:
+  int was_ = 0, now_ = 0;
+};
+
+}  // namespace
+}  // namespace chonk
+
+using namespace chonk;
+
+extern "C" {
+
+int64_t chonk_kv_page_bytes(int32_t kv_type, int32_t kv_heads, int32_t head_dim) {
+  int64_t n = 0;
+  const int rc = api_free([&] {
+    check_format(kv_type, kv_heads, head_dim);
+    n = (int64_t)kv_heads * 2 * kv_part_bytes(kv_type, head_dim);
+  });
+  return rc == CHONK_OK ? n : rc;
+}
+
+int chonk_kv_append(const chonk_kv_cache* cache, const chonk_kv_rows* rows, const chonk_kv_append_args* x,
+                    void* stream) {
+  return api_free([&] {
+    KvAppendArgs a{};
+    a.c = checked(cache);
+    if (!rows || !x) throw Error(CHONK_EINVAL, "null argument");
+    check_rows(rows->n);
+    check_act(x->type);
+    if (rows->n == 0) return;
+    if (!rows->seq || !rows->pos || !x->k || !x->v) throw Error(CHONK_EINVAL, "null argument");
+    const int64_t kvw = (int64_t)a.c.kv_heads * a.c.hd;
+    check_stride("k", x->k_stride, kvw);
+    check_stride("v", x->v_stride, kvw);
+    if (x->q) {
+      check_heads(x->heads, a.c.kv_heads);
+      if (!x->q_out) throw Error(CHONK_EINVAL, "null argument");
+      check_stride("q", x->q_stride, (int64_t)x->heads * a.c.hd);
+      check_stride("q_out", x->q_out_stride, (int64_t)x->heads * a.c.hd);
+    }
+    if (x->rope && (x->rope_dim <= 0 || x->rope_dim > a.c.hd || x->rope_dim % 2 || x->rope_positions <= 0))
+      throw Error(CHONK_EINVAL, no("paged K/V cache: rope_dim must be even and at most head_dim, not", x->rope_dim));
+    if (x->k_norm || x->q_norm) {
+      if (!(x->eps >= 0.0)) throw Error(CHONK_EINVAL, "paged K/V cache: eps must not be negative");
+    }
+    check_grid((int64_t)rows->n * ((x->q ? x->heads : 0) + a.c.kv_heads + 3) / 4);
+    a.at.seq = rows->seq;
+    a.at.pos = rows->pos;
+    a.rows = rows->n;
+    a.heads = x->heads;
+    a.f16 = x->type == CHONK_F16;
+    a.q_ld = x->q_stride;
+    a.k_ld = x->k_stride;
+    a.v_ld = x->v_stride;
+    a.qo_ld = x->q_out_stride;
+    a.q_out = x->q_out;
+    if (a.f16) {
+      a.q16 = (const _Float16*)x->q;
+      a.k16 = (const _Float16*)x->k;
+      a.v16 = (const _Float16*)x->v;
+    } else {
+      const void* src[3] = {x->q, x->k, x->v};
+      const int64_t ld[3] = {x->q_stride, x->k_stride, x->v_stride};
+      PartSum* dst[3] = {&a.q, &a.k, &a.v};
+      for (int i = 0; i < 3; ++i) {
+        if (ld[i] > INT32_MAX) throw Error(CHONK_EINVAL, "paged K/V cache: rows are too far apart");
+        dst[i]->p = (const float*)src[i];
+        dst[i]->ks = 1;
+        dst[i]->ld = (int32_t)ld[i];
+      }
+    }
+    a.qn_w = x->q_norm;
+    a.kn_w = x->k_norm;
+    a.eps = x->eps;
+    a.rope = (const float2*)x->rope;
+    a.rope_dim = x->rope_dim;
+    a.rope_n = x->rope_positions;
+    a.interleaved = x->interleaved != 0;
+    OnDevice on(cache->device);
+    HIP_OK(launch_kv_append(a, (hipStream_t)stream));
+  });
+}
+
+int chonk_kv_read(const chonk_kv_cache* cache, const chonk_kv_rows* rows, int32_t type, void* k, void* v,
+                  int64_t row_stride, int64_t head_stride, void* stream) {
+  return api_free([&] {
+    KvReadArgs a{};
+    a.c = checked(cache);
+    if (!rows || (!k && !v)) throw Error(CHONK_EINVAL, "null argument");
+    check_rows(rows->n);
+    check_act(type);
+    if (rows->n == 0) return;
+    if (!rows->seq || !rows->pos) throw Error(CHONK_EINVAL, "null argument");
+    // either order of rows and heads, none inside another
+    const int64_t hd = a.c.hd;
+    const bool rows_out = head_stride >= hd && row_stride >= (a.c.kv_heads - 1) * head_stride + hd;
+    const bool heads_out = row_stride >= hd && head_stride >= (int64_t)(rows->n - 1) * row_stride + hd;
+    if (!rows_out && !heads_out) throw Error(CHONK_EINVAL, "paged K/V cache: result rows overlap");
+    check_grid((int64_t)rows->n * a.c.kv_heads * (a.c.hd / 8) / kWg);
+    a.at.seq = rows->seq;
+    a.at.pos = rows->pos;
+    a.rows = rows->n;
+    a.k = k;
+    a.v = v;
+    a.row_ld = row_stride;
+    a.head_ld = head_stride;
+    a.f16 = type == CHONK_F16;
+    OnDevice on(cache->device);
+    HIP_OK(launch_kv_read(a, (hipStream_t)stream));
+  });
+}
+
+int64_t chonk_kv_attend_workspace(const chonk_kv_cache* cache, int32_t n_rows, int32_t heads) {
+  int64_t n = 0;
+  const int rc = api_free([&] {
+    const KvCache c = checked(cache);
+    check_rows(n_rows);
+    check_heads(heads, c.kv_heads);
+    n = n_rows ? kv_attend_floats(c, n_rows, heads) * 4 : 0;
+  });
+  return rc == CHONK_OK ? n : rc;
+}
+
+int chonk_kv_attend(const chonk_kv_cache* cache, const chonk_kv_attend_args* x, void* stream) {
+  return api_free([&] {
+    KvAttendArgs a{};
+    a.c = checked(cache);
+    if (!x) throw Error(CHONK_EINVAL, "null argument");
+    check_rows(x->n);
+    check_act(x->type);
+    check_heads(x->heads, a.c.kv_heads);
+    if (x->window < 0) throw Error(CHONK_EINVAL, no("paged K/V cache: bad window", x->window));
+    if (x->n == 0) return;
+    if (!x->seq || !x->lengths || !x->q || !x->out) throw Error(CHONK_EINVAL, "null argument");
+    check_stride("q", x->q_stride, (int64_t)x->heads * a.c.hd);
+    check_stride("out", x->out_stride, (int64_t)x->heads * a.c.hd);
+    const int G = x->heads / a.c.kv_heads;
+    check_grid((int64_t)x->n * a.c.kv_heads * ((G + 15) / 16) + kWantWgs);
+    const int64_t need = kv_attend_floats(a.c, x->n, x->heads) * 4;
+    if (need > 0 && (!x->workspace || x->workspace_bytes < need || (uintptr_t)x->workspace % 16))
+      throw Error(CHONK_EINVAL, "paged K/V cache: attention needs " + std::to_string(need) +
+                                    " bytes of 16-byte aligned workspace, got " + std::to_string(x->workspace_bytes));
+    a.seq = x->seq;
+    a.len = x->lengths;
+    a.q = x->q;
+    a.out = x->out;
+    a.q_ld = x->q_stride;
+    a.o_ld = x->out_stride;
+    a.rows = x->n;
+    a.heads = x->heads;
+    a.f16 = x->type == CHONK_F16;
+    a.window = x->window;
+    a.scale = x->scale;
+    a.part = (float*)x->workspace;
+    OnDevice on(cache->device);
+    HIP_OK(launch_kv_attend(a, (hipStream_t)stream));
+  });
+}
+
+}  // extern "C"

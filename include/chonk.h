@@ -59,6 +59,8 @@ extern "C" {
 
 #define CHONK_KV_F16 0       /* fp16 K/V cache (default) */
 #define CHONK_KV_F32 1       /* fp32 K/V cache, the reference layout (:830-831) */
+#define CHONK_KV_Q8 2        /* 8-bit codes, one fp16 scale per 32 dims (paged caches) */
+#define CHONK_KV_Q4 3        /* 4-bit codes, one fp16 scale per 32 dims (paged caches) */
 
 typedef struct chonk_engine chonk_engine;
 
@@ -251,6 +253,108 @@ int chonk_batch_step(chonk_batch* b, const int32_t* seqs, const int32_t* tokens,
 int chonk_batch_position(const chonk_batch* b, int32_t seq, int32_t* out_pos);
 /* Logits of row `row` of the last prefill (row 0) or step. */
 int chonk_batch_read_logits(chonk_batch* b, int32_t row, float* out, size_t n);
+
+/* Paged K/V cache operators (no counterpart in the reference) ---------------------
+ * For programs that keep K and V of many sequences in pages of 64 positions and
+ * drive the layers themselves. All pointers below are device memory of
+ * cache->device that the caller owns; a call checks its arguments, enqueues on
+ * `stream` (a hipStream_t; NULL: the default stream) and returns without
+ * waiting. Calls may be captured into a HIP graph. Nothing is kept between calls.
+ *
+ * Values. CHONK_KV_F16: fp16. CHONK_KV_Q8 / _Q4: each block of 32 dims of a
+ * position and head has an fp16 scale d and codes c, and stands for d * c.
+ *   Q8: d = fp16(max |x| / 127),  c = rint(x / d) in [-127, 127]
+ *   Q4: d = fp16(m / -8), m the element of largest magnitude (the first of
+ *       equals), c = rint(x / d) in [-8, 7]
+ * (rint to even; d saturates at 65504; d = 0 gives codes 0). A block with a NaN or
+ * an infinity gets d = NaN: all of it reads back as NaN.
+ *
+ * Pages. Per kv head: K codes | K scales | V codes | V scales. Codes come in units of
+ * 32 positions (half u of the page) x 32 dims (block b), units in the order
+ * [u][b]; inside a unit (n = 16 g + i, 0 <= g < 4, 0 <= i < 16):
+ *   K: dims 8 g .. 8 g + 7 of position 16 t + i
+ *   V: positions 4 g + (e % 4) + 16 (e / 4), e = 0 .. 7, of dim 16 h + i
+ *   F16: 8 halves at [t][n] (V: [h][n])
+ *   Q8:  8 bytes code + 128 at [n][t] (V: [n][h])
+ *   Q4:  K 4 bytes at [n][t], dims 8 g + m and 8 g + m + 4 in the low and high
+ *        nibble of byte m as code + 8; V 8 bytes at [n], dims i and 16 + i in
+ *        the low and high nibble of byte e
+ * Scales are [u][b][32], place 8 g + e for position 4 g + (e % 4) + 16 (e / 4).
+ *
+ * Rows that name no place of the cache: a negative sequence leaves a row out
+ * (its result stays as it was). A sequence past n_seqs, a position past the
+ * table's (or the rotary table's) end or a table entry outside the pool is refused by the
+ * kernel: nothing is written for that row (chonk_kv_attend: its result is NaN)
+ * and the bits 1 (sequence), 2 (position), 4 (page) are set in *fault. */
+#define CHONK_F32 0
+#define CHONK_F16 1
+
+typedef struct {
+  int32_t kv_type;          /* CHONK_KV_F16, CHONK_KV_Q8 or CHONK_KV_Q4 */
+  int32_t kv_heads;
+  int32_t head_dim;         /* 32, 64, 128 or 256 */
+  int32_t n_pages;
+  void* pages;              /* n_pages * chonk_kv_page_bytes, 16-byte aligned */
+  int32_t n_seqs, max_pages;
+  const int32_t* table;     /* [n_seqs][max_pages] page of each 64 positions */
+  int32_t* fault;           /* one word, or NULL */
+  int32_t device;
+} chonk_kv_cache;
+
+typedef struct {
+  int32_t n;
+  const int32_t* seq;       /* [n] */
+  const int32_t* pos;       /* [n] */
+} chonk_kv_rows;
+
+typedef struct {
+  int32_t type;             /* CHONK_F32 or CHONK_F16: of q, k, v and q_out */
+  int32_t heads;            /* query heads (a multiple of the kv heads); not read without q */
+  const void *q, *k, *v;    /* [n][heads][head_dim], [n][kv_heads][head_dim]; q may be NULL */
+  void* q_out;              /* may be q */
+  int64_t q_stride, k_stride, v_stride, q_out_stride;  /* elements from row to row */
+  const float *q_norm, *k_norm;  /* RMSNorm weights [head_dim], or NULL */
+  double eps;
+  const float* rope;        /* (cos, sin) [rope_positions][rope_dim / 2][2], or NULL */
+  int32_t rope_dim, rope_positions;
+  int32_t interleaved;      /* rotary pairs (2 i, 2 i + 1) instead of (i, i + rope_dim / 2) */
+} chonk_kv_append_args;
+
+typedef struct {
+  int32_t type;             /* CHONK_F32 or CHONK_F16: of q and out */
+  int32_t heads;
+  int32_t n;
+  const int32_t* seq;       /* [n] */
+  const int32_t* lengths;   /* [n] positions of the sequence that the row sees */
+  const void* q;            /* [n][heads][head_dim] */
+  void* out;                /* [n][heads][head_dim] */
+  int64_t q_stride, out_stride;
+  float scale;
+  int32_t window;           /* the last `window` of those positions alone; 0: all */
+  void* workspace;          /* chonk_kv_attend_workspace bytes; of one call at a time */
+  int64_t workspace_bytes;
+} chonk_kv_attend_args;
+
+/* Bytes of one page, or a negative status. */
+int64_t chonk_kv_page_bytes(int32_t kv_type, int32_t kv_heads, int32_t head_dim);
+/* Writes row i's k and v to position pos[i] of sequence seq[i], and q to q_out: q and k
+ * through an RMSNorm of every head (x / sqrt(mean x^2 + eps) * w) and the rotary
+ * embedding of the row's position, where given. Rows name distinct places (what
+ * lies in a place named twice is a mixture). The codes are functions of the row alone: of
+ * fp32 products and sums rounded one by one and a sum of squares in 64 bits. */
+int chonk_kv_append(const chonk_kv_cache* cache, const chonk_kv_rows* rows, const chonk_kv_append_args* args,
+                    void* stream);
+/* The values stored at the rows' places: k and v (either may be NULL) of type
+ * `type`, element (i, head, dim) at i * row_stride + head * head_stride + dim. */
+int chonk_kv_read(const chonk_kv_cache* cache, const chonk_kv_rows* rows, int32_t type, void* k, void* v,
+                  int64_t row_stride, int64_t head_stride, void* stream);
+/* Bytes of workspace of chonk_kv_attend for n_rows rows, or a negative status. */
+int64_t chonk_kv_attend_workspace(const chonk_kv_cache* cache, int32_t n_rows, int32_t heads);
+/* Attention of one query token a row: out = softmax(scale * q K^T) V over the
+ * positions [max(0, length - window), length) of the row's sequence, query head h over kv
+ * head h / (heads / kv_heads). A length of 0 or less gives zeros. Several rows may name
+ * one sequence. The result does not depend on what lies in other positions. */
+int chonk_kv_attend(const chonk_kv_cache* cache, const chonk_kv_attend_args* args, void* stream);
 
 /* Kernel-level entry points (tests) ---------------------------------------
  * GGUF rows are given as raw block bytes in host memory; the call uploads
