@@ -63,7 +63,8 @@ struct KvAttendArgs {
   const void* q;
   void* out;
   int64_t q_ld, o_ld;
-  int32_t rows, heads, f16, vec, window, nseg;
+  int32_t rows, heads, f16, window;
+  int32_t split;          // set by the launcher: rows are cut into segments, joined from part
   float scale;
   float* part;
 };

@@ -31,6 +31,9 @@ typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
+constexpr int kWantWgs = 1024;  // segments of a split attention (four workgroups a CU)
+constexpr int kMinHalves = 16;  // ... of at least so many half pages
+
 __device__ __forceinline__ f4_t mfma(h8_t a, h8_t b, f4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
@@ -333,39 +336,195 @@ constexpr int kOrder(int e) {  // element e of an operand's k: which of the eigh
   return o[e];
 }
 
-// One workgroup per (row, kv head, up to 16 of its q heads, segment of the
-// row's pages); its four waves take the pages in turn, each with its own running
+// One half page (32 positions) of a head's K or V in a lane's registers.
+template <int KV, int NB>
+struct Codes {
+  static constexpr int kWords = KV == CHONK_KV_F16 ? 8 : KV == CHONK_KV_Q8 ? 4 : 2;  // a block
+  uint32_t w[NB * kWords];
+  uint32_t d[NB == 8 ? 2 : 1];  // the half's scales, two (four) of its 32 NB a lane
+
+  __device__ __forceinline__ void load(const uint8_t* part, int u, int lane) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const uint8_t* unit = part + (u * NB + b) * (kv_code_bytes(KV, 32) / 2);
+      if constexpr (KV == CHONK_KV_Q4) {
+        const uint2 x = ldg2(unit + lane * 8);
+        w[2 * b] = x.x, w[2 * b + 1] = x.y;
+      } else {
+#pragma unroll
+        for (int t = 0; t < kWords / 4; ++t) {
+          const uint4 x = ldg4(unit + t * 1024 + lane * 16);
+          w[kWords * b + 4 * t] = x.x, w[kWords * b + 4 * t + 1] = x.y;
+          w[kWords * b + 4 * t + 2] = x.z, w[kWords * b + 4 * t + 3] = x.w;
+        }
+      }
+    }
+    if constexpr (KV != CHONK_KV_F16) {
+      const uint8_t* s = part + kv_code_bytes(KV, 32 * NB) + u * NB * 64;
+      if constexpr (NB == 8) {
+        const uint2 x = ldg2(s + lane * 8);
+        d[0] = x.x, d[1] = x.y;
+      } else {
+        d[0] = ldg1(s + (lane & (NB * 16 - 1)) * 4);
+      }
+    }
+  }
+  // The A operands of block b: K's two tiles of 16 positions, V's two of 16 dims.
+  __device__ __forceinline__ void tiles(int b, bool is_v, h8_t& a0, h8_t& a1) const {
+    const uint32_t* x = w + kWords * b;
+    if constexpr (KV == CHONK_KV_F16) {
+      a0 = __builtin_bit_cast(h8_t, u32x4_t{x[0], x[1], x[2], x[3]});
+      a1 = __builtin_bit_cast(h8_t, u32x4_t{x[4], x[5], x[6], x[7]});
+    } else if constexpr (KV == CHONK_KV_Q8) {
+      a0 = codes8(x[0], x[1]);
+      a1 = codes8(x[2], x[3]);
+    } else if (is_v) {
+      a0 = join(nibbles4<0>(x[0]), nibbles4<0>(x[1]));
+      a1 = join(nibbles4<1>(x[0]), nibbles4<1>(x[1]));
+    } else {
+      a0 = join(nibbles4<0>(x[0]), nibbles4<1>(x[0]));
+      a1 = join(nibbles4<0>(x[1]), nibbles4<1>(x[1]));
+    }
+  }
+};
+
+// A row's visible positions, as half pages.
+struct Span {
+  int seq, len, first, h0, h1;
+  bool bad;
+  __device__ __forceinline__ Span(const KvAttendArgs& a, int seq_, int len_, bool note) : seq(seq_), len(len_ + a.len_add) {
+    bad = seq >= 0 && len > 0 && (seq >= a.c.n_seqs || len > a.c.max_pages * kKvPage);
+    if (bad && note) fault(a.c, seq >= a.c.n_seqs ? KVF_SEQ : KVF_POS);
+    if (bad || seq < 0) len = 0;
+    len = max(len, 0);
+    first = a.window > 0 ? max(0, len - a.window) : 0;
+    h0 = first / 32;
+    h1 = (len + 31) / 32;
+  }
+};
+
+// The rows' cut into segments, the same in every workgroup: at most kWantWgs
+// segments of at most `most` halves, found from all the rows' lengths, so that ragged rows
+// keep the device as evenly busy as equal ones and the host needs to know no
+// length. Rows (at most kWg) are the threads'; the thread that `mine` holds for
+// leaves its row's index, segments before it and segments in pick[0..2].
+template <class F>
+__device__ __forceinline__ void cut_rows(const KvAttendArgs& a, int items_per_row, int* tmp, int* pick, F mine) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  int n = 0;
+  if (t < a.rows) {
+    const Span s(a, a.seq[t], a.len[t], false);
+    n = s.h1 - s.h0;
+  }
+  int sum = n;
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
+  if (lane == 0) tmp[wave] = sum;
+  __syncthreads();
+  // (in 64 bits: 256 rows of 2^25 halves, times the heads)
+  const int64_t total = ((int64_t)tmp[0] + tmp[1] + tmp[2] + tmp[3]) * items_per_row;
+  const int64_t room = kWantWgs - a.rows * items_per_row;
+  const int64_t most = max((int64_t)kMinHalves, (total + room - 1) / room);
+  const int segs = t < a.rows ? max(1, (int)((n + most - 1) / most)) : 0;
+  int before = segs;
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) {
+    const int o = __shfl_up(before, x);
+    if (lane >= x) before += o;
+  }
+  __syncthreads();
+  if (lane == 63) tmp[wave] = before;
+  __syncthreads();
+  before -= segs;
+  for (int w = 0; w < wave; ++w) before += tmp[w];
+  if (t < a.rows && mine(t, before, segs)) {
+    pick[0] = t;
+    pick[1] = before;
+    pick[2] = segs;
+  }
+  __syncthreads();
+}
+
+// w * half H of d: the sum with 0 makes it one mixed instruction. (Not in asm: w
+// comes from an exponential, whose result the next instruction cannot take
+// without a wait that the compiler sees to.)
+template <int H>
+__device__ __forceinline__ float mul_half(float w, uint32_t d) {
+  return fmaf((float)__builtin_bit_cast(h2_t, d)[H], w, 0.f);
+}
+// w less half H of h, in one instruction. h is a conversion's result, w that or what the
+// conversion took, so neither is an exponential's fresh one.
+template <int H>
+__device__ __forceinline__ float less_half(float w, uint32_t h) {
+  float o;
+  if constexpr (H == 0)
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(o) : "v"(h), "v"(w));
+  else
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(o) : "v"(h), "v"(w));
+  return o;
+}
+// Two weights as fp16 pairs hi + lo (22 bits; both cut, the second from what the first leaves).
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+  lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(less_half<0>(x, hi), less_half<1>(y, hi)));
+}
+
+// One workgroup per segment of a (row, kv head, up to 16 of its q heads); its
+// four waves take the segment's half pages in turn, each with its own running
 // maximum, sum and output, and meet in LDS at the end.
 template <int KV, int NB>
-__global__ __launch_bounds__(kWg) void k_kv_attend(KvAttendArgs a) {
+__global__ __launch_bounds__(kWg, NB == 8 ? 1 : NB == 4 ? 2 : 3) void k_kv_attend(KvAttendArgs a) {
   constexpr int HD = 32 * NB;
-  constexpr int CODES = kv_code_bytes(KV, HD), PART = kv_part_bytes(KV, HD);
-  constexpr int UNIT = CODES / (2 * NB);
+  constexpr int PART = kv_part_bytes(KV, HD);
   extern __shared__ __align__(16) float sm[];  // [wave][head][HD] | [wave][head][m, l]
-  const int G = a.heads / a.c.kv_heads, hgs = (G + 15) / 16;
-  int id = blockIdx.x;
-  const int seg = id % a.nseg;
-  id /= a.nseg;
-  const int hg = id % hgs;
-  id /= hgs;
-  const int kv = id % a.c.kv_heads, r = id / a.c.kv_heads;
-  const int h0 = kv * G + hg * 16, nh = min(16, G - hg * 16);
+  __shared__ int tmp[4], pick[3];
+  __shared__ __align__(16) uint32_t scl[4][2][NB * 16];
+  const int G = a.heads / a.c.kv_heads, hgs = (G + 15) / 16, items = a.c.kv_heads * hgs;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, col = lane & 15;
-
-  const int seq = ld_scalar(a.seq + r);
-  if (seq < 0) return;  // (the join leaves the row alone too)
-  int len = ld_scalar(a.len + r) + a.len_add;
-  bool bad = false;
-  if (len > 0 && (seq >= a.c.n_seqs || len > a.c.max_pages * kKvPage)) {
-    if (tid == 0) fault(a.c, seq >= a.c.n_seqs ? KVF_SEQ : KVF_POS);
-    bad = true;
-    len = 0;
+  int r, it, seg = 0, segs = 1;
+  if (a.split) {
+    if (tid == 0) pick[0] = -1;
+    const int id = blockIdx.x;
+    cut_rows(a, items, tmp, pick, [&](int, int before, int n) { return id >= before * items && id < (before + n) * items; });
+    r = __builtin_amdgcn_readfirstlane(pick[0]);
+    if (r < 0) return;
+    segs = __builtin_amdgcn_readfirstlane(pick[2]);
+    const int x = id - __builtin_amdgcn_readfirstlane(pick[1]) * items;
+    it = x / segs;
+    seg = x % segs;
+  } else {
+    r = blockIdx.x / items;
+    it = blockIdx.x % items;
   }
-  const int first = a.window > 0 ? max(0, len - a.window) : 0;
-  const int pg0 = first / kKvPage, pg1 = (max(len, 0) + kKvPage - 1) / kKvPage;
-  const int per = (pg1 - pg0 + a.nseg - 1) / a.nseg;
-  const int from = pg0 + seg * per, to = min(from + per, pg1);
+  const int kv = it / hgs, hg = it % hgs;
+  const int h0 = kv * G + hg * 16, nh = min(16, G - hg * 16);
+  const Span sp(a, ld_scalar(a.seq + r), ld_scalar(a.len + r), tid == 0);
+  if (sp.seq < 0) return;  // (the join leaves the row alone too)
+  const int per = (sp.h1 - sp.h0 + segs - 1) / segs;
+  const int to = min(sp.h0 + (seg + 1) * per, sp.h1);
+  int hx = sp.h0 + seg * per + wave;
+
+  // the first half page's K and V are on their way before anything else
+  const int32_t* tab = a.c.table + (size_t)sp.seq * a.c.max_pages;
+  const uint8_t* pool = a.c.pages + (size_t)kv * 2 * PART;
+  const size_t page_bytes = (size_t)a.c.kv_heads * 2 * PART;
+  bool poison = sp.bad;
+  auto part_of = [&](int h) {
+    int page = ld_scalar(tab + h / 2);
+    if (page < 0 || page >= a.c.n_pages) {
+      if (lane == 0) fault(a.c, KVF_PAGE);
+      poison = true;
+      page = 0;
+    }
+    return pool + (size_t)page * page_bytes;
+  };
+  Codes<KV, NB> kc, vc;
+  if (hx < to) {
+    const uint8_t* p = part_of(hx);
+    kc.load(p, hx & 1, lane);
+    vc.load(p + PART, hx & 1, lane);
+  }
 
   // q: this lane's head at dims 32 b + 8 g + e, scaled by a power of two so that the
   // head's largest lies in [2^13, 2^14) and split into two halves of 11 bits each
@@ -389,158 +548,152 @@ __global__ __launch_bounds__(kWg) void k_kv_attend(KvAttendArgs a) {
     top = fmaxf(t0, t1);
     swap32(top, t0, t1);
     top = fmaxf(t0, t1);
-    const int sh = top > 0.f ? min(13 - ilogbf(top), 100) : 0;
-    mul = ldexpf(a.scale * 1.44269504f, -sh);
+    // (a power of two of the head's largest, and the sign of the scale, into q: mul is positive)
+    const int sh = top > 0.f ? min(13 - ((int)(__float_as_uint(top) >> 23) - 127), 100) : 0;
+    mul = a.scale == 0.f ? 1.f : ldexpf(fabsf(a.scale) * 1.44269504f, -sh);
+    const float f = a.scale == 0.f ? 0.f : copysignf(ldexpf(1.f, sh), a.scale);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         // (the high nibbles are 16 times their code)
-        const float y = ldexpf(x[b][e], sh - (KV == CHONK_KV_Q4 && e >= 4 ? 4 : 0));
+        const float y = x[b][e] * (KV == CHONK_KV_Q4 && e >= 4 ? f * 0.0625f : f);
         qh[b][e] = (_Float16)y;
         ql[b][e] = (_Float16)(y - (float)qh[b][e]);
       }
   }
 
-  // m is the reference of the exponents: the running maximum mx less an offset
-  // that keeps weight * V scale within fp16 and its bits above fp16's denormals
-  float mx = -1e30f, m = -1e30f, l = 0.f, dtop = 0.f, off = KV == CHONK_KV_F16 ? 14.f : 0.f;
+  // m is the reference of the exponents: the running maximum mx less an offset that
+  // keeps weight * V scale below 2^14 and its bits above fp16's denormals; dtop is the largest
+  // exponent of a V scale so far
+  float mx = -1e30f, m = -1e30f, l = 0.f;
+  int dtop = 0;
   f4_t acc[2 * NB];
 #pragma unroll
   for (int i = 0; i < 2 * NB; ++i) acc[i] = f4_t{0.f, 0.f, 0.f, 0.f};
 
-  for (int pg = from + wave; pg < to; pg += 4) {
-    const int page = ld_scalar(a.c.table + (size_t)seq * a.c.max_pages + pg);
-    if (page < 0 || page >= a.c.n_pages) {
-      if (lane == 0) fault(a.c, KVF_PAGE);
-      l = __builtin_nanf("");
-      continue;
-    }
-    const uint8_t* kb = a.c.pages + ((size_t)page * a.c.kv_heads + kv) * 2 * PART;
-    const uint8_t* vb = kb + PART;
+  for (; hx < to; hx += 4) {
+    const int j0 = 32 * hx;
+    const bool edge = j0 < sp.first || j0 + 32 > sp.len;
+    const bool more = hx + 4 < to;
+    if constexpr (KV != CHONK_KV_F16) {
+      if (edge) {  // scales of unseen places may be anything
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int j0 = pg * kKvPage + 32 * u;
-      if (j0 >= len || j0 + 32 <= first) continue;
-      float s[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s[e] = 0.f;
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const uint8_t* unit = kb + (u * NB + b) * UNIT;
-        h8_t k0, k1;
-        if constexpr (KV == CHONK_KV_F16) {
-          k0 = __builtin_bit_cast(h8_t, ldg4(unit + lane * 16));
-          k1 = __builtin_bit_cast(h8_t, ldg4(unit + 1024 + lane * 16));
-        } else if constexpr (KV == CHONK_KV_Q8) {
-          const uint4 w = ldg4(unit + lane * 16);
-          k0 = codes8(w.x, w.y);
-          k1 = codes8(w.z, w.w);
-        } else {
-          const uint2 w = ldg2(unit + lane * 8);
-          k0 = join(nibbles4<0>(w.x), nibbles4<1>(w.x));
-          k1 = join(nibbles4<0>(w.y), nibbles4<1>(w.y));
-        }
-        const f4_t z = f4_t{0.f, 0.f, 0.f, 0.f};
-        const f4_t s0 = mfma(k0, ql[b], mfma(k0, qh[b], z));
-        const f4_t s1 = mfma(k1, ql[b], mfma(k1, qh[b], z));
-        if constexpr (KV == CHONK_KV_F16) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[e] += s0[e];
-            s[4 + e] += s1[e];
-          }
-        } else {
-          const h8_t d = __builtin_bit_cast(h8_t, ldg4(kb + CODES + (u * NB + b) * 64 + g * 16));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[e] = fmaf((float)d[e], s0[e], s[e]);
-            s[4 + e] = fmaf((float)d[4 + e], s1[e], s[4 + e]);
-          }
+        for (int i = 0; i < (NB == 8 ? 2 : 1); ++i) {
+          const int n = ((NB == 8 ? 2 * lane + i : lane) & 15) * 2;  // place of the word's first
+          const int j = j0 + 4 * (n >> 3) + (n & 3) + 16 * ((n >> 2) & 1);
+          if (j < sp.first || j >= sp.len) vc.d[i] &= 0xffff0000u;
+          if (j + 1 < sp.first || j + 1 >= sp.len) vc.d[i] &= 0xffffu;
         }
       }
-      float top = -1e30f;
-      bool out[8];
+      if constexpr (NB == 8) {
+        *(uint2*)(scl[wave][0] + 2 * lane) = make_uint2(kc.d[0], kc.d[1]);
+        *(uint2*)(scl[wave][1] + 2 * lane) = make_uint2(vc.d[0], vc.d[1]);
+      } else if (lane < NB * 16) {
+        scl[wave][0][lane] = kc.d[0];
+        scl[wave][1][lane] = vc.d[0];
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    float s[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      h8_t k0, k1;
+      kc.tiles(b, false, k0, k1);
+      const f4_t z = f4_t{0.f, 0.f, 0.f, 0.f};
+      const f4_t s0 = mfma(k0, ql[b], mfma(k0, qh[b], z));
+      const f4_t s1 = mfma(k1, ql[b], mfma(k1, qh[b], z));
+      if constexpr (KV == CHONK_KV_F16) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[e] += s0[e];
+          s[4 + e] += s1[e];
+        }
+      } else {
+        const h8_t d = *(const h8_t*)(scl[wave][0] + b * 16 + g * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[e] = fmaf((float)d[e], s0[e], s[e]);
+          s[4 + e] = fmaf((float)d[4 + e], s1[e], s[4 + e]);
+        }
+      }
+    }
+    const uint8_t* next = more ? part_of(hx + 4) : nullptr;
+    if (more) kc.load(next, hx & 1, lane);  // (4 halves on: the same half of its page)
+    uint32_t seen[4];  // of the pairs of places, for fp16 V
+    if (edge) {
+      uint32_t out = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int j = j0 + 4 * g + (e & 3) + 16 * (e >> 2);
-        out[e] = j < first || j >= len;
-        s[e] = out[e] ? -INFINITY : s[e] * mul;
-        top = fmaxf(top, s[e]);
+        const bool o = j < sp.first || j >= sp.len;
+        out |= (uint32_t)o << e;
+        s[e] = o ? -INFINITY : s[e];
       }
-      float t0, t1;
-      swap16(top, t0, t1);
-      top = fmaxf(t0, t1);
-      swap32(top, t0, t1);
-      top = fmaxf(t0, t1);
-      h8_t dv[NB];
-      if constexpr (KV != CHONK_KV_F16) {
-        // the largest scale so far bounds weight * scale
-        float dm = 0.f;
+      if constexpr (KV == CHONK_KV_F16) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          dv[b] = __builtin_bit_cast(h8_t, ldg4(vb + CODES + (u * NB + b) * 64 + g * 16));
+        for (int i = 0; i < 4; ++i) seen[i] = (out >> (2 * i) & 1 ? 0 : 0xffffu) | (out >> (2 * i + 1) & 1 ? 0 : 0xffff0000u);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) dm = fmaxf(dm, out[e] ? 0.f : fabsf((float)dv[b][e]));
-        }
-        swap16(dm, t0, t1);
-        dm = fmaxf(t0, t1);
-        swap32(dm, t0, t1);
-        dm = fminf(fmaxf(t0, t1), 65504.f);
-        if (dm > dtop) {
-          dtop = dm;
-          off = (float)(13 - ilogbf(dtop));  // weight * scale < 2^14
-        }
-      }
-      mx = fmaxf(mx, top);
-      const float ref = mx - off;
-      if (__ballot(ref != m)) {
-        const float f = exp2f(m - ref);
-        l *= f;
-#pragma unroll
-        for (int i = 0; i < 2 * NB; ++i) acc[i] *= f;
-        m = ref;
-      }
-      float p[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        p[e] = out[e] ? 0.f : exp2f(s[e] - m);
-        l += p[e];
-      }
-#pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        h8_t ph, pl;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int k = kOrder<KV>(e);
-          float w = p[k];
-          if constexpr (KV != CHONK_KV_F16) w = out[k] ? 0.f : w * (float)dv[b][k];
-          ph[e] = (_Float16)w;
-          pl[e] = (_Float16)(w - (float)ph[e]);
-        }
-        const uint8_t* unit = vb + (u * NB + b) * UNIT;
-        h8_t v0, v1;
-        if constexpr (KV == CHONK_KV_F16) {
-          v0 = __builtin_bit_cast(h8_t, ldg4(unit + lane * 16));
-          v1 = __builtin_bit_cast(h8_t, ldg4(unit + 1024 + lane * 16));
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {  // (what lies in unseen places may be anything)
-            v0[e] = out[e] ? (_Float16)0 : v0[e];
-            v1[e] = out[e] ? (_Float16)0 : v1[e];
-          }
-        } else if constexpr (KV == CHONK_KV_Q8) {
-          const uint4 w = ldg4(unit + lane * 16);
-          v0 = codes8(w.x, w.y);
-          v1 = codes8(w.z, w.w);
-        } else {
-          const uint2 w = ldg2(unit + lane * 8);
-          v0 = join(nibbles4<0>(w.x), nibbles4<0>(w.y));
-          v1 = join(nibbles4<1>(w.x), nibbles4<1>(w.y));
-        }
-        acc[2 * b] = mfma(v0, pl, mfma(v0, ph, acc[2 * b]));
-        acc[2 * b + 1] = mfma(v1, pl, mfma(v1, ph, acc[2 * b + 1]));
+        for (int i = 0; i < NB * 8; ++i) vc.w[i] &= seen[i & 3];
       }
     }
+    float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+    float t0, t1;
+    swap16(top, t0, t1);
+    top = fmaxf(t0, t1);
+    swap32(top, t0, t1);
+    mx = fmaxf(mx, fmaxf(t0, t1) * mul);
+    float off = 14.f;
+    if constexpr (KV != CHONK_KV_F16) {
+      uint32_t x = 0;
+#pragma unroll
+      for (int i = 0; i < (NB == 8 ? 2 : 1); ++i) {
+        const uint32_t lo = vc.d[i] & 0x7fffu, hi = vc.d[i] >> 16 & 0x7fffu;
+        x = max(x, max(lo > 0x7bffu ? 0 : lo, hi > 0x7bffu ? 0 : hi));
+      }
+      x = (uint32_t)wave_max((float)x);
+      dtop = max(dtop, (int)__builtin_amdgcn_readfirstlane(x) >> 10);
+      off = (float)(28 - dtop);
+    }
+    const float ref = mx - off;
+    if (__ballot(ref != m)) {
+      const float f = __builtin_amdgcn_exp2f(m - ref);
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < 2 * NB; ++i) acc[i] *= f;
+      m = ref;
+    }
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], mul, -m));
+      l += p[e];
+    }
+    uint32_t ph[4], pl[4];
+    if constexpr (KV == CHONK_KV_F16) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) split2(p[2 * i], p[2 * i + 1], ph[i], pl[i]);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      if constexpr (KV != CHONK_KV_F16) {
+        const uint4 d = *(const uint4*)(scl[wave][1] + b * 16 + g * 4);
+        split2(mul_half<0>(p[0], d.x), mul_half<0>(p[2], d.y), ph[0], pl[0]);
+        split2(mul_half<1>(p[1], d.x), mul_half<1>(p[3], d.y), ph[1], pl[1]);
+        split2(mul_half<0>(p[4], d.z), mul_half<0>(p[6], d.w), ph[2], pl[2]);
+        split2(mul_half<1>(p[5], d.z), mul_half<1>(p[7], d.w), ph[3], pl[3]);
+      }
+      const h8_t wh = __builtin_bit_cast(h8_t, u32x4_t{ph[0], ph[1], ph[2], ph[3]});
+      const h8_t wl = __builtin_bit_cast(h8_t, u32x4_t{pl[0], pl[1], pl[2], pl[3]});
+      h8_t v0, v1;
+      vc.tiles(b, true, v0, v1);
+      acc[2 * b] = mfma(v0, wl, mfma(v0, wh, acc[2 * b]));
+      acc[2 * b + 1] = mfma(v1, wl, mfma(v1, wh, acc[2 * b + 1]));
+    }
+    if (more) vc.load(next + PART, hx & 1, lane);
   }
   {
     float t0, t1;
@@ -549,7 +702,7 @@ __global__ __launch_bounds__(kWg) void k_kv_attend(KvAttendArgs a) {
     swap32(l, t0, t1);
     l = t0 + t1;
   }
-  if (bad) l = __builtin_nanf("");
+  if (poison) l = __builtin_nanf("");
   // the waves' rows meet in LDS
   float* ml = sm + 4 * nh * HD;
   if (col < nh) {
@@ -566,6 +719,8 @@ __global__ __launch_bounds__(kWg) void k_kv_attend(KvAttendArgs a) {
     }
   }
   __syncthreads();
+  float* prow = a.part + (int64_t)blockIdx.x * min(G, 16) * HD;
+  float* pml = a.part + (int64_t)kWantWgs * min(G, 16) * HD + (int64_t)blockIdx.x * min(G, 16) * 2;
   for (int x = tid; x < nh * HD; x += kWg) {
     const int h = x / HD, d = x % HD;
     float M = -1e30f;
@@ -574,16 +729,15 @@ __global__ __launch_bounds__(kWg) void k_kv_attend(KvAttendArgs a) {
     float L = 0.f, O = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float f = exp2f(ml[(w * nh + h) * 2] - M);
+      const float f = __builtin_amdgcn_exp2f(ml[(w * nh + h) * 2] - M);
       L += f * ml[(w * nh + h) * 2 + 1];
       O += f * sm[(w * nh + h) * HD + d];
     }
-    if (a.nseg > 1) {
-      float* p = a.part + (((int64_t)r * a.heads + h0 + h) * a.nseg + seg) * (HD + 2);
-      p[d] = O;
+    if (segs > 1) {
+      prow[x] = O;
       if (d == 0) {
-        p[HD] = M;
-        p[HD + 1] = L;
+        pml[2 * h] = M;
+        pml[2 * h + 1] = L;
       }
     } else {
       const float y = L == 0.f ? 0.f : O / L;
@@ -596,32 +750,63 @@ __global__ __launch_bounds__(kWg) void k_kv_attend(KvAttendArgs a) {
   }
 }
 
-// Joins a (row, head)'s segments, in their order.
+// Joins a (row, head)'s segments: HD / 4 columns of float4, the segments over
+// groups of threads, every group's in order and the groups in order.
 __global__ __launch_bounds__(kWg) void k_kv_join(KvAttendArgs a) {
-  const int h = blockIdx.x, r = blockIdx.y, hd = a.c.hd, d = threadIdx.x;
-  if (d >= hd || a.seq[r] < 0) return;
-  const float* p = a.part + ((int64_t)r * a.heads + h) * a.nseg * (hd + 2);
+  __shared__ int tmp[4], pick[3];
+  __shared__ float wt[kWantWgs];
+  __shared__ float red[8];
+  __shared__ __align__(16) float so[kWg * 4];
+  const int G = a.heads / a.c.kv_heads, hgs = (G + 15) / 16, items = a.c.kv_heads * hgs, nhm = min(G, 16);
+  const int h = blockIdx.x, r = blockIdx.y, hd = a.c.hd, tid = threadIdx.x;
+  cut_rows(a, items, tmp, pick, [&](int t, int, int) { return t == r; });
+  const int segs = pick[2];
+  if (segs == 1) return;
+  const int it = h / G * hgs + h % G / 16, hh = h % G % 16;
+  const int slot0 = pick[1] * items + it * segs;
+  const float* rows = a.part + ((int64_t)slot0 * nhm + hh) * hd;
+  const float* ml = a.part + (int64_t)kWantWgs * nhm * hd + ((int64_t)slot0 * nhm + hh) * 2;
   float M = -1e30f;
-  for (int s = 0; s < a.nseg; ++s) M = fmaxf(M, p[s * (hd + 2) + hd]);
-  float L = 0.f, O = 0.f;
-  for (int s = 0; s < a.nseg; ++s) {
-    const float f = exp2f(p[s * (hd + 2) + hd] - M);
-    L += f * p[s * (hd + 2) + hd + 1];
-    O += f * p[s * (hd + 2) + d];
+  for (int s = tid; s < segs; s += kWg) M = fmaxf(M, ml[(int64_t)s * nhm * 2]);
+  M = wave_max(M);
+  if ((tid & 63) == 0) red[tid >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float L = 0.f;
+  for (int s = tid; s < segs; s += kWg) {
+    const float f = __builtin_amdgcn_exp2f(ml[(int64_t)s * nhm * 2] - M);
+    wt[s] = f;
+    L += f * ml[(int64_t)s * nhm * 2 + 1];
   }
-  const float y = L == 0.f ? 0.f : O / L;
-  const int64_t o = r * a.o_ld + (int64_t)h * hd + d;
-  if (a.f16)
-    ((_Float16*)a.out)[o] = (_Float16)y;
-  else
-    ((float*)a.out)[o] = y;
+  L = wave_sum(L);
+  if ((tid & 63) == 0) red[4 + (tid >> 6)] = L;
+  __syncthreads();
+  L = (red[4] + red[5]) + (red[6] + red[7]);
+  const int cols = hd / 4, c = tid % cols, grp = tid / cols, groups = kWg / cols;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int s = grp; s < segs; s += groups) {
+    const float4 v = ldg4f(rows + (int64_t)s * nhm * hd + 4 * c);
+    const float f = wt[s];
+    o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+  }
+  *(float4*)(so + 4 * tid) = o;
+  __syncthreads();
+  for (int d = tid; d < hd; d += kWg) {
+    float y = 0.f;
+    for (int g = 0; g < groups; ++g) y += so[4 * (g * cols) + d];
+    y = L == 0.f ? 0.f : y / L;
+    const int64_t at = r * a.o_ld + (int64_t)h * hd + d;
+    if (a.f16)
+      ((_Float16*)a.out)[at] = (_Float16)y;
+    else
+      ((float*)a.out)[at] = y;
+  }
 }
 
-constexpr int kWantWgs = 1024;
-
-int attend_segments(const KvCache& c, int rows, int heads) {
+bool attend_splits(const KvCache& c, int rows, int heads) {
   const int64_t n = (int64_t)rows * c.kv_heads * ((heads / c.kv_heads + 15) / 16);
-  return (int)std::max<int64_t>(1, std::min<int64_t>((c.max_pages + 3) / 4, kWantWgs / n));
+  return rows <= kWg && n <= kWantWgs / 2 && 2 * c.max_pages > kMinHalves;
 }
 
 }  // namespace
@@ -665,16 +850,15 @@ hipError_t launch_kv_read(const KvReadArgs& a, hipStream_t s) {
 }
 
 int64_t kv_attend_floats(const KvCache& c, int rows, int heads) {
-  const int nseg = attend_segments(c, rows, heads);
-  return nseg > 1 ? (int64_t)rows * heads * nseg * (c.hd + 2) : 0;
+  return attend_splits(c, rows, heads) ? (int64_t)kWantWgs * std::min(heads / c.kv_heads, 16) * (c.hd + 2) : 0;
 }
 
 hipError_t launch_kv_attend(const KvAttendArgs& a0, hipStream_t s) {
   KvAttendArgs a = a0;
   const int G = a.heads / a.c.kv_heads, hgs = (G + 15) / 16, nh = std::min(G, 16);
-  a.nseg = attend_segments(a.c, a.rows, a.heads);
-  if (a.nseg > 1 && !a.part) return hipErrorInvalidValue;
-  const dim3 grid((uint32_t)((int64_t)a.rows * a.c.kv_heads * hgs * a.nseg));
+  a.split = attend_splits(a.c, a.rows, a.heads) ? 1 : 0;
+  if (a.split && !a.part) return hipErrorInvalidValue;
+  const dim3 grid(a.split ? kWantWgs : (uint32_t)((int64_t)a.rows * a.c.kv_heads * hgs));
   const size_t sh = (size_t)4 * nh * (a.c.hd + 2) * 4;
 #define CHONK_KV_CASE(T, B)                                                                              \
   if (a.c.type == T && a.c.hd == 32 * B) {                                                               \
@@ -699,7 +883,7 @@ hipError_t launch_kv_attend(const KvAttendArgs& a0, hipStream_t s) {
   CHONK_KV_CASE(CHONK_KV_Q4, 8)
   return hipErrorInvalidValue;
 #undef CHONK_KV_CASE
-  if (a.nseg > 1) hipLaunchKernelGGL(k_kv_join, dim3(a.heads, a.rows), dim3(kWg), 0, s, a);
+  if (a.split) hipLaunchKernelGGL(k_kv_join, dim3(a.heads, a.rows), dim3(kWg), 0, s, a);
   return hipGetLastError();
 }
 
@@ -905,7 +1089,7 @@ int chonk_kv_attend(const chonk_kv_cache* cache, const chonk_kv_attend_args* x, 
     check_stride("q", x->q_stride, (int64_t)x->heads * a.c.hd);
     check_stride("out", x->out_stride, (int64_t)x->heads * a.c.hd);
     const int G = x->heads / a.c.kv_heads;
-    check_grid((int64_t)x->n * a.c.kv_heads * ((G + 15) / 16) + kWantWgs);
+    check_grid((int64_t)x->n * a.c.kv_heads * ((G + 15) / 16));
     const int64_t need = kv_attend_floats(a.c, x->n, x->heads) * 4;
     if (need > 0 && (!x->workspace || x->workspace_bytes < need || (uintptr_t)x->workspace % 16))
       throw Error(CHONK_EINVAL, "paged K/V cache: attention needs " + std::to_string(need) +
