@@ -64,7 +64,7 @@ struct KvAttendArgs {
   void* out;
   int64_t q_ld, o_ld;
   int32_t rows, heads, f16, window;
-  int32_t split;          // set by the launcher: rows are cut into segments, joined from part
+  int32_t split, want;    // set by the launcher: rows are cut into at most `want` segments, joined from part
   float scale;
   float* part;
 };

@@ -31,7 +31,7 @@ typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kWantWgs = 1024;  // segments of a split attention (four workgroups a CU)
+constexpr int kMostWgs = 1024;  // segments of a split attention, at most
 constexpr int kMinHalves = 16;  // ... of at least so many half pages
 
 __device__ __forceinline__ f4_t mfma(h8_t a, h8_t b, f4_t c) {
@@ -304,30 +304,37 @@ __global__ __launch_bounds__(kWg) void k_kv_read(KvReadArgs a) {
 
 // ---- attention --------------------------------------------------------------------
 
-// Eight codes as exact halves. Bytes come through v_perm beside 0x64 (1024 + c
-// is exact in fp16) and the bias goes in one packed subtraction, so the halves'
-// order is (0, 2, 1, 3, 4, 6, 5, 7): both products take their k in that order.
-__device__ __forceinline__ h2_t bias2(uint32_t v, float b) {
-  const _Float16 h = (_Float16)b;
-  return __builtin_bit_cast(h2_t, v) - h2_t{h, h};
+// Codes become exact fp16 operands two at a time: put under the exponent of 1024,
+// where the last bit counts 1 (bytes by v_perm beside 0x64, nibbles by an and with an
+// or; 16 times the code for high nibbles), and 1024 and the bias subtracted, exactly.
+// Bytes 0 and 2 of a word share a register, and 1 and 3, so the order of eight is
+// (0, 2, 1, 3, 4, 6, 5, 7): both products take their k in that order.
+// (As denormals, one operation for two codes, the matrix unit takes them too; but it
+// aligns such a product by the exponent 2^-14 that denormals share, and a code of b bits
+// loses 10 - b of the product's 24: results were off by 1e-5 with 4 bits, and by
+// 2.5e-6 instead of 5e-7 with 8, for 4 us of 22 at 41k positions.)
+__device__ __forceinline__ uint32_t less2(uint32_t v, uint32_t k) {
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2_t, v) - __builtin_bit_cast(h2_t, k));
 }
-__device__ __forceinline__ h8_t codes8(uint32_t w0, uint32_t w1) {
-  constexpr uint32_t kE = 0x64646464u;
-  const h2_t a = bias2(__builtin_amdgcn_perm(kE, w0, 0x04020400u), 1152.f);
-  const h2_t b = bias2(__builtin_amdgcn_perm(kE, w0, 0x04030401u), 1152.f);
-  const h2_t c = bias2(__builtin_amdgcn_perm(kE, w1, 0x04020400u), 1152.f);
-  const h2_t d = bias2(__builtin_amdgcn_perm(kE, w1, 0x04030401u), 1152.f);
-  return h8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+__device__ __forceinline__ uint32_t even_bytes(uint32_t w) {
+  return less2(__builtin_amdgcn_perm(0x64646464u, w, 0x04020400u), 0x64806480u);
 }
-// The low (H = 0) or high nibbles of the words' bytes; the high ones as 16 times the code.
-template <int H>
-__device__ __forceinline__ h4_t nibbles4(uint32_t w) {
-  constexpr uint32_t kM = H ? 0x00f000f0u : 0x000f000fu;
-  const float b = H ? 1152.f : 1032.f;
-  const h2_t x = bias2((w & kM) | 0x64006400u, b), y = bias2(((w >> 8) & kM) | 0x64006400u, b);
-  return h4_t{x[0], x[1], y[0], y[1]};
+__device__ __forceinline__ uint32_t odd_bytes(uint32_t w) {
+  return less2(__builtin_amdgcn_perm(0x64646464u, w, 0x04030401u), 0x64806480u);
 }
-__device__ __forceinline__ h8_t join(h4_t a, h4_t b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
+__device__ __forceinline__ uint32_t low_nibbles(uint32_t w) {
+  uint32_t e = 0x64006400u;
+  asm("" : "+v"(e));  // (a register: with two literals the and and the or would be two instructions)
+  return less2((w & 0x000f000fu) | e, 0x64086408u);
+}
+__device__ __forceinline__ uint32_t high_nibbles(uint32_t w) {
+  uint32_t e = 0x64006400u;
+  asm("" : "+v"(e));
+  return less2((w & 0x00f000f0u) | e, 0x64806480u);
+}
+__device__ __forceinline__ h8_t halves(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __builtin_bit_cast(h8_t, u32x4_t{a, b, c, d});
+}
 
 template <int KV>
 constexpr int kOrder(int e) {  // element e of an operand's k: which of the eight
@@ -370,20 +377,29 @@ struct Codes {
     }
   }
   // The A operands of block b: K's two tiles of 16 positions, V's two of 16 dims.
-  __device__ __forceinline__ void tiles(int b, bool is_v, h8_t& a0, h8_t& a1) const {
+  // High nibbles are 16 times their code.
+  __device__ __forceinline__ void k_tiles(int b, h8_t& a0, h8_t& a1) const {
     const uint32_t* x = w + kWords * b;
     if constexpr (KV == CHONK_KV_F16) {
-      a0 = __builtin_bit_cast(h8_t, u32x4_t{x[0], x[1], x[2], x[3]});
-      a1 = __builtin_bit_cast(h8_t, u32x4_t{x[4], x[5], x[6], x[7]});
+      a0 = halves(x[0], x[1], x[2], x[3]);
+      a1 = halves(x[4], x[5], x[6], x[7]);
     } else if constexpr (KV == CHONK_KV_Q8) {
-      a0 = codes8(x[0], x[1]);
-      a1 = codes8(x[2], x[3]);
-    } else if (is_v) {
-      a0 = join(nibbles4<0>(x[0]), nibbles4<0>(x[1]));
-      a1 = join(nibbles4<1>(x[0]), nibbles4<1>(x[1]));
+      a0 = halves(even_bytes(x[0]), odd_bytes(x[0]), even_bytes(x[1]), odd_bytes(x[1]));
+      a1 = halves(even_bytes(x[2]), odd_bytes(x[2]), even_bytes(x[3]), odd_bytes(x[3]));
     } else {
-      a0 = join(nibbles4<0>(x[0]), nibbles4<1>(x[0]));
-      a1 = join(nibbles4<0>(x[1]), nibbles4<1>(x[1]));
+      const uint32_t y0 = x[0] >> 8, y1 = x[1] >> 8;
+      a0 = halves(low_nibbles(x[0]), low_nibbles(y0), high_nibbles(x[0]), high_nibbles(y0));
+      a1 = halves(low_nibbles(x[1]), low_nibbles(y1), high_nibbles(x[1]), high_nibbles(y1));
+    }
+  }
+  __device__ __forceinline__ void v_tiles(int b, h8_t& a0, h8_t& a1) const {
+    if constexpr (KV == CHONK_KV_Q4) {
+      const uint32_t* x = w + kWords * b;
+      const uint32_t y0 = x[0] >> 8, y1 = x[1] >> 8;
+      a0 = halves(low_nibbles(x[0]), low_nibbles(y0), low_nibbles(x[1]), low_nibbles(y1));
+      a1 = halves(high_nibbles(x[0]), high_nibbles(y0), high_nibbles(x[1]), high_nibbles(y1));
+    } else {
+      k_tiles(b, a0, a1);
     }
   }
 };
@@ -403,46 +419,62 @@ struct Span {
   }
 };
 
-// The rows' cut into segments, the same in every workgroup: at most kWantWgs
-// segments of at most `most` halves, found from all the rows' lengths, so that ragged rows
-// keep the device as evenly busy as equal ones and the host needs to know no
-// length. Rows (at most kWg) are the threads'; the thread that `mine` holds for
-// leaves its row's index, segments before it and segments in pick[0..2].
+// The rows' cut into segments, the same in every wave: at most `want`
+// segments of about as many halves each, found from all the rows' lengths, so that
+// ragged rows keep the device as evenly busy as equal ones and the host needs to know no
+// length. A lane looks at rows 4 lane .. 4 lane + 3 (at most 256 rows). The row that
+// `mine` holds for comes back in all lanes (row -1: none).
+struct Cut {
+  int row, seq, len, before, segs;  // segments of the rows before it (an item each), segments of its items
+};
 template <class F>
-__device__ __forceinline__ void cut_rows(const KvAttendArgs& a, int items_per_row, int* tmp, int* pick, F mine) {
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  int n = 0;
-  if (t < a.rows) {
-    const Span s(a, a.seq[t], a.len[t], false);
-    n = s.h1 - s.h0;
-  }
-  int sum = n;
+__device__ __forceinline__ Cut cut_rows(const KvAttendArgs& a, int items, F mine) {
+  constexpr int R = 4;
+  const int lane = threadIdx.x & 63, r0 = R * lane;
+  int seq[R], len[R], n[R], sum = 0;
 #pragma unroll
-  for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
-  if (lane == 0) tmp[wave] = sum;
-  __syncthreads();
-  // (in 64 bits: 256 rows of 2^25 halves, times the heads)
-  const int64_t total = ((int64_t)tmp[0] + tmp[1] + tmp[2] + tmp[3]) * items_per_row;
-  const int64_t room = kWantWgs - a.rows * items_per_row;
-  const int64_t most = max((int64_t)kMinHalves, (total + room - 1) / room);
-  const int segs = t < a.rows ? max(1, (int)((n + most - 1) / most)) : 0;
-  int before = segs;
+  for (int i = 0; i < R; ++i) {
+    const int r = min(r0 + i, a.rows - 1);
+    seq[i] = a.seq[r];
+    len[i] = a.len[r];
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const Span s(a, seq[i], len[i], false);
+    n[i] = r0 + i < a.rows ? s.h1 - s.h0 : 0;
+  }
+  // (as floats: a bound that is a little off only makes segments a little longer)
+  float total = 0.f;
+#pragma unroll
+  for (int i = 0; i < R; ++i) total += (float)n[i];
+  total = wave_sum(total) * (float)items;
+  const int room = a.want - a.rows * items;
+  const int most = max(kMinHalves, (int)fminf(total / (float)room * 1.0001f + 1.f, 1e9f));
+  int segs[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    segs[i] = r0 + i < a.rows ? max(1, (int)((uint32_t)(n[i] + most - 1) / (uint32_t)most)) : 0;
+    sum += segs[i];
+  }
+  int before = sum;
 #pragma unroll
   for (int x = 1; x < 64; x *= 2) {
     const int o = __shfl_up(before, x);
     if (lane >= x) before += o;
   }
-  __syncthreads();
-  if (lane == 63) tmp[wave] = before;
-  __syncthreads();
-  before -= segs;
-  for (int w = 0; w < wave; ++w) before += tmp[w];
-  if (t < a.rows && mine(t, before, segs)) {
-    pick[0] = t;
-    pick[1] = before;
-    pick[2] = segs;
+  before -= sum;
+  Cut c{-1, 0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (r0 + i < a.rows && mine(r0 + i, before, segs[i])) c = Cut{r0 + i, seq[i], len[i], before, segs[i]};
+    before += segs[i];
   }
-  __syncthreads();
+  const uint64_t found = __ballot(c.row >= 0);
+  if (!found) return Cut{-1, 0, 0, 0, 0};
+  const int at = __builtin_ctzll(found);
+  return Cut{__builtin_amdgcn_readlane(c.row, at), __builtin_amdgcn_readlane(c.seq, at),
+             __builtin_amdgcn_readlane(c.len, at), __builtin_amdgcn_readlane(c.before, at),
+             __builtin_amdgcn_readlane(c.segs, at)};
 }
 
 // w * half H of d: the sum with 0 makes it one mixed instruction. (Not in asm: w
@@ -472,34 +504,47 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 // One workgroup per segment of a (row, kv head, up to 16 of its q heads); its
 // four waves take the segment's half pages in turn, each with its own running
 // maximum, sum and output, and meet in LDS at the end.
-template <int KV, int NB>
-__global__ __launch_bounds__(kWg, NB == 8 ? 1 : NB == 4 ? 2 : 3) void k_kv_attend(KvAttendArgs a) {
-  constexpr int HD = 32 * NB;
-  constexpr int PART = kv_part_bytes(KV, HD);
+//
+// PACK (at most four heads): the products have 16 columns for them, and what is done to
+// the scores between the products (exponentials, weights times V's scales,
+// their split into two halves) would be done on all 16. So the scores of a half
+// page, 4 heads x 32 positions, go through LDS to two a lane, and the split
+// weights back; the idle columns get a copy of the others.
+template <int KV, int NB, bool PACK>
+__global__ __launch_bounds__(kWg, NB == 8 ? 2 : NB == 4 ? 3 : 4) void k_kv_attend(KvAttendArgs a) {
+  constexpr int HD = 32 * NB, PART = kv_part_bytes(KV, HD);
+  constexpr bool F = KV == CHONK_KV_F16;
+  constexpr int WB = F ? 1 : NB;            // blocks with weights of their own
+  // What registers cannot hold beside K and V of a half page and the output: q's halves
+  // go to LDS, and fp16's 256-wide rows are fetched one of K and V at a time.
+  constexpr bool QL = NB == 8 || (NB == 4 && KV != CHONK_KV_Q4);
+  constexpr bool ONE = F && NB == 8;
   extern __shared__ __align__(16) float sm[];  // [wave][head][HD] | [wave][head][m, l]
-  __shared__ int tmp[4], pick[3];
-  __shared__ __align__(16) uint32_t scl[4][2][NB * 16];
+  __shared__ __align__(16) uint32_t sck[4][F ? 4 : NB * 16];          // K's scales, as stored
+  __shared__ __align__(16) uint32_t scv[4][F ? 4 : NB * 16];          // V's (PACK: [pair][block])
+  __shared__ __align__(16) float ss[4][PACK ? 4 * 32 : 4];            // scores [head][place]
+  __shared__ __align__(16) uint32_t sw[4][PACK ? WB * 2 * 64 : 4];    // weights [block][hi, lo][head][16 pairs]
+  __shared__ __align__(16) uint32_t sq[QL ? NB * 2 * 64 * 4 : 4];
   const int G = a.heads / a.c.kv_heads, hgs = (G + 15) / 16, items = a.c.kv_heads * hgs;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, col = lane & 15;
-  int r, it, seg = 0, segs = 1;
+  int r, it, seq, len, seg = 0, segs = 1;
   if (a.split) {
-    if (tid == 0) pick[0] = -1;
     const int id = blockIdx.x;
-    cut_rows(a, items, tmp, pick, [&](int, int before, int n) { return id >= before * items && id < (before + n) * items; });
-    r = __builtin_amdgcn_readfirstlane(pick[0]);
-    if (r < 0) return;
-    segs = __builtin_amdgcn_readfirstlane(pick[2]);
-    const int x = id - __builtin_amdgcn_readfirstlane(pick[1]) * items;
-    it = x / segs;
-    seg = x % segs;
+    const Cut c = cut_rows(a, items, [&](int, int before, int n) { return id >= before * items && id < (before + n) * items; });
+    if (c.row < 0) return;
+    r = c.row, seq = c.seq, len = c.len, segs = c.segs;
+    it = (id - c.before * items) / segs;
+    seg = (id - c.before * items) % segs;
   } else {
     r = blockIdx.x / items;
     it = blockIdx.x % items;
+    seq = ld_scalar(a.seq + r);
+    len = ld_scalar(a.len + r);
   }
   const int kv = it / hgs, hg = it % hgs;
   const int h0 = kv * G + hg * 16, nh = min(16, G - hg * 16);
-  const Span sp(a, ld_scalar(a.seq + r), ld_scalar(a.len + r), tid == 0);
+  const Span sp(a, seq, len, tid == 0);
   if (sp.seq < 0) return;  // (the join leaves the row alone too)
   const int per = (sp.h1 - sp.h0 + segs - 1) / segs;
   const int to = min(sp.h0 + (seg + 1) * per, sp.h1);
@@ -523,13 +568,13 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 1 : NB == 4 ? 2 : 3) void k_kv_atten
   if (hx < to) {
     const uint8_t* p = part_of(hx);
     kc.load(p, hx & 1, lane);
-    vc.load(p + PART, hx & 1, lane);
+    if constexpr (!ONE) vc.load(p + PART, hx & 1, lane);
   }
 
   // q: this lane's head at dims 32 b + 8 g + e, scaled by a power of two so that the
   // head's largest lies in [2^13, 2^14) and split into two halves of 11 bits each
-  h8_t qh[NB], ql[NB];
-  float mul;  // score of S in powers of two
+  h8_t qh[QL ? 1 : NB], ql[QL ? 1 : NB];
+  float mul;             // score of S in powers of two
   {
     float x[NB][8];
     const int h = h0 + min(col, nh - 1);
@@ -553,15 +598,33 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 1 : NB == 4 ? 2 : 3) void k_kv_atten
     mul = a.scale == 0.f ? 1.f : ldexpf(fabsf(a.scale) * 1.44269504f, -sh);
     const float f = a.scale == 0.f ? 0.f : copysignf(ldexpf(1.f, sh), a.scale);
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b) {
+      h8_t hi, lo;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        // (the high nibbles are 16 times their code)
-        const float y = x[b][e] * (KV == CHONK_KV_Q4 && e >= 4 ? f * 0.0625f : f);
-        qh[b][e] = (_Float16)y;
-        ql[b][e] = (_Float16)(y - (float)qh[b][e]);
+        const float part = KV == CHONK_KV_Q4 && e >= 4 ? 0.0625f : 1.f;  // (high nibbles are 16 times their code)
+        const float y = x[b][e] * f * part;
+        hi[e] = (_Float16)y;
+        lo[e] = (_Float16)(y - (float)hi[e]);
       }
+      if constexpr (QL) {
+        if (wave == 0) {
+          *(h8_t*)(sq + (2 * b * 64 + lane) * 4) = hi;
+          *(h8_t*)(sq + ((2 * b + 1) * 64 + lane) * 4) = lo;
+        }
+      } else {
+        qh[b] = hi;
+        ql[b] = lo;
+      }
+    }
   }
+  if constexpr (QL) __syncthreads();
+
+  // With PACK a lane's two scores are head `hc`'s at places pa and pb, the pair
+  // pc of the 16 that make up the second product's operand.
+  const int hc = lane >> 4, pc = lane & 15;
+  const int pa = F ? 2 * pc : 8 * (pc >> 2) + (pc & 1) + 4 * ((pc >> 1) & 1), pb = pa + (F ? 1 : 2);
+  if constexpr (PACK) mul = __shfl(mul, hc);
 
   // m is the reference of the exponents: the running maximum mx less an offset that
   // keeps weight * V scale below 2^14 and its bits above fp16's denormals; dtop is the largest
@@ -576,22 +639,37 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 1 : NB == 4 ? 2 : 3) void k_kv_atten
     const int j0 = 32 * hx;
     const bool edge = j0 < sp.first || j0 + 32 > sp.len;
     const bool more = hx + 4 < to;
-    if constexpr (KV != CHONK_KV_F16) {
+    if constexpr (!F) {
+      constexpr int D = NB == 8 ? 2 : 1;
       if (edge) {  // scales of unseen places may be anything
 #pragma unroll
-        for (int i = 0; i < (NB == 8 ? 2 : 1); ++i) {
-          const int n = ((NB == 8 ? 2 * lane + i : lane) & 15) * 2;  // place of the word's first
+        for (int i = 0; i < D; ++i) {
+          const int n = ((D * lane + i) & 15) * 2;  // place of the word's first
           const int j = j0 + 4 * (n >> 3) + (n & 3) + 16 * ((n >> 2) & 1);
           if (j < sp.first || j >= sp.len) vc.d[i] &= 0xffff0000u;
           if (j + 1 < sp.first || j + 1 >= sp.len) vc.d[i] &= 0xffffu;
         }
       }
+      // (PACK: the words re-paired as the weights are, (0, 2), (1, 3) of each four)
       if constexpr (NB == 8) {
-        *(uint2*)(scl[wave][0] + 2 * lane) = make_uint2(kc.d[0], kc.d[1]);
-        *(uint2*)(scl[wave][1] + 2 * lane) = make_uint2(vc.d[0], vc.d[1]);
-      } else if (lane < NB * 16) {
-        scl[wave][0][lane] = kc.d[0];
-        scl[wave][1][lane] = vc.d[0];
+        *(uint2*)(sck[wave] + 2 * lane) = make_uint2(kc.d[0], kc.d[1]);
+        if constexpr (PACK) {
+          uint32_t* o = scv[wave] + (2 * lane & 15) * NB + (lane >> 3);
+          o[0] = __builtin_amdgcn_perm(vc.d[1], vc.d[0], 0x05040100u);
+          o[NB] = __builtin_amdgcn_perm(vc.d[1], vc.d[0], 0x07060302u);
+        } else {
+          *(uint2*)(scv[wave] + 2 * lane) = make_uint2(vc.d[0], vc.d[1]);
+        }
+      } else {
+        uint32_t v = vc.d[0];
+        if constexpr (PACK) {
+          const uint32_t w = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, false);
+          v = __builtin_amdgcn_perm(w, v, lane & 1 ? 0x03020706u : 0x05040100u);
+        }
+        if (lane < NB * 16) {
+          sck[wave][lane] = kc.d[0];
+          scv[wave][PACK ? (lane & 15) * NB + (lane >> 4) : lane] = v;
+        }
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -601,19 +679,26 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 1 : NB == 4 ? 2 : 3) void k_kv_atten
     for (int e = 0; e < 8; ++e) s[e] = 0.f;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      h8_t k0, k1;
-      kc.tiles(b, false, k0, k1);
+      h8_t k0, k1, hi, lo;
+      kc.k_tiles(b, k0, k1);
+      if constexpr (QL) {
+        hi = *(const h8_t*)(sq + (2 * b * 64 + lane) * 4);
+        lo = *(const h8_t*)(sq + ((2 * b + 1) * 64 + lane) * 4);
+      } else {
+        hi = qh[b];
+        lo = ql[b];
+      }
       const f4_t z = f4_t{0.f, 0.f, 0.f, 0.f};
-      const f4_t s0 = mfma(k0, ql[b], mfma(k0, qh[b], z));
-      const f4_t s1 = mfma(k1, ql[b], mfma(k1, qh[b], z));
-      if constexpr (KV == CHONK_KV_F16) {
+      const f4_t s0 = mfma(k0, lo, mfma(k0, hi, z));
+      const f4_t s1 = mfma(k1, lo, mfma(k1, hi, z));
+      if constexpr (F) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[e] += s0[e];
           s[4 + e] += s1[e];
         }
       } else {
-        const h8_t d = *(const h8_t*)(scl[wave][0] + b * 16 + g * 4);
+        const h8_t d = *(const h8_t*)(sck[wave] + b * 16 + g * 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           s[e] = fmaf((float)d[e], s0[e], s[e]);
@@ -621,9 +706,12 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 1 : NB == 4 ? 2 : 3) void k_kv_atten
         }
       }
     }
-    const uint8_t* next = more ? part_of(hx + 4) : nullptr;
-    if (more) kc.load(next, hx & 1, lane);  // (4 halves on: the same half of its page)
-    uint32_t seen[4];  // of the pairs of places, for fp16 V
+    // (4 halves on: the same half of its page)
+    const uint8_t* next = ONE ? part_of(hx) : more ? part_of(hx + 4) : nullptr;
+    if constexpr (ONE)
+      vc.load(next + PART, hx & 1, lane);
+    else if (more)
+      kc.load(next, hx & 1, lane);
     if (edge) {
       uint32_t out = 0;
 #pragma unroll
@@ -633,21 +721,16 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 1 : NB == 4 ? 2 : 3) void k_kv_atten
         out |= (uint32_t)o << e;
         s[e] = o ? -INFINITY : s[e];
       }
-      if constexpr (KV == CHONK_KV_F16) {
+      if constexpr (F) {
+        uint32_t seen[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) seen[i] = (out >> (2 * i) & 1 ? 0 : 0xffffu) | (out >> (2 * i + 1) & 1 ? 0 : 0xffff0000u);
 #pragma unroll
         for (int i = 0; i < NB * 8; ++i) vc.w[i] &= seen[i & 3];
       }
     }
-    float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-    float t0, t1;
-    swap16(top, t0, t1);
-    top = fmaxf(t0, t1);
-    swap32(top, t0, t1);
-    mx = fmaxf(mx, fmaxf(t0, t1) * mul);
     float off = 14.f;
-    if constexpr (KV != CHONK_KV_F16) {
+    if constexpr (!F) {
       uint32_t x = 0;
 #pragma unroll
       for (int i = 0; i < (NB == 8 ? 2 : 1); ++i) {
@@ -658,44 +741,100 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 1 : NB == 4 ? 2 : 3) void k_kv_atten
       dtop = max(dtop, (int)__builtin_amdgcn_readfirstlane(x) >> 10);
       off = (float)(28 - dtop);
     }
+    float s0 = 0.f, s1 = 0.f, top;
+    if constexpr (PACK) {
+      if (col < 4) {
+        *(float4*)(ss[wave] + col * 32 + 8 * g) = make_float4(s[0], s[1], s[2], s[3]);
+        *(float4*)(ss[wave] + col * 32 + 8 * g + 4) = make_float4(s[4], s[5], s[6], s[7]);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      s0 = ss[wave][hc * 32 + pa];
+      s1 = ss[wave][hc * 32 + pb];
+      top = group_max<16>(fmaxf(s0, s1));
+    } else {
+      top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+      float t0, t1;
+      swap16(top, t0, t1);
+      top = fmaxf(t0, t1);
+      swap32(top, t0, t1);
+      top = fmaxf(t0, t1);
+    }
+    mx = fmaxf(mx, top * mul);
     const float ref = mx - off;
     if (__ballot(ref != m)) {
       const float f = __builtin_amdgcn_exp2f(m - ref);
       l *= f;
-#pragma unroll
-      for (int i = 0; i < 2 * NB; ++i) acc[i] *= f;
       m = ref;
-    }
-    float p[8];
+      const float fa = PACK ? __shfl(f, (col & 3) * 16) : f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], mul, -m));
-      l += p[e];
+      for (int i = 0; i < 2 * NB; ++i) acc[i] *= fa;
+    }
+    float p[PACK ? 2 : 8];
+    if constexpr (PACK) {
+      p[0] = __builtin_amdgcn_exp2f(fmaf(s0, mul, -m));
+      p[1] = __builtin_amdgcn_exp2f(fmaf(s1, mul, -m));
+      l += p[0] + p[1];
+      uint32_t dv[NB];
+      if constexpr (!F) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) dv[b] = scv[wave][pc * NB + b];
+      }
+#pragma unroll
+      for (int b = 0; b < WB; ++b) {
+        uint32_t hi, lo;
+        if constexpr (F)
+          split2(p[0], p[1], hi, lo);
+        else
+          split2(mul_half<0>(p[0], dv[b]), mul_half<1>(p[1], dv[b]), hi, lo);
+        sw[wave][2 * b * 64 + lane] = hi;
+        sw[wave][(2 * b + 1) * 64 + lane] = lo;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], mul, -m));
+        l += p[e];
+      }
     }
     uint32_t ph[4], pl[4];
-    if constexpr (KV == CHONK_KV_F16) {
+    if constexpr (F && !PACK) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) split2(p[2 * i], p[2 * i + 1], ph[i], pl[i]);
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      if constexpr (KV != CHONK_KV_F16) {
-        const uint4 d = *(const uint4*)(scl[wave][1] + b * 16 + g * 4);
-        split2(mul_half<0>(p[0], d.x), mul_half<0>(p[2], d.y), ph[0], pl[0]);
-        split2(mul_half<1>(p[1], d.x), mul_half<1>(p[3], d.y), ph[1], pl[1]);
-        split2(mul_half<0>(p[4], d.z), mul_half<0>(p[6], d.w), ph[2], pl[2]);
-        split2(mul_half<1>(p[5], d.z), mul_half<1>(p[7], d.w), ph[3], pl[3]);
+      h8_t wh, wl, v0, v1;
+      if constexpr (PACK) {
+        const uint32_t* x = sw[wave] + 2 * (F ? 0 : b) * 64 + (col & 3) * 16 + 4 * g;
+        wh = *(const h8_t*)x;
+        wl = *(const h8_t*)(x + 64);
+      } else {
+        if constexpr (!F) {
+          const uint4 d = *(const uint4*)(scv[wave] + b * 16 + g * 4);
+          split2(mul_half<0>(p[0], d.x), mul_half<0>(p[2], d.y), ph[0], pl[0]);
+          split2(mul_half<1>(p[1], d.x), mul_half<1>(p[3], d.y), ph[1], pl[1]);
+          split2(mul_half<0>(p[4], d.z), mul_half<0>(p[6], d.w), ph[2], pl[2]);
+          split2(mul_half<1>(p[5], d.z), mul_half<1>(p[7], d.w), ph[3], pl[3]);
+        }
+        wh = halves(ph[0], ph[1], ph[2], ph[3]);
+        wl = halves(pl[0], pl[1], pl[2], pl[3]);
       }
-      const h8_t wh = __builtin_bit_cast(h8_t, u32x4_t{ph[0], ph[1], ph[2], ph[3]});
-      const h8_t wl = __builtin_bit_cast(h8_t, u32x4_t{pl[0], pl[1], pl[2], pl[3]});
-      h8_t v0, v1;
-      vc.tiles(b, true, v0, v1);
+      vc.v_tiles(b, v0, v1);
       acc[2 * b] = mfma(v0, wl, mfma(v0, wh, acc[2 * b]));
       acc[2 * b + 1] = mfma(v1, wl, mfma(v1, wh, acc[2 * b + 1]));
     }
-    if (more) vc.load(next + PART, hx & 1, lane);
+    if constexpr (ONE) {
+      if (more) kc.load(part_of(hx + 4), hx & 1, lane);
+    } else if (more) {
+      vc.load(next + PART, hx & 1, lane);
+    }
   }
-  {
+  if constexpr (PACK) {
+    l = group_sum<16>(l);
+  } else {
     float t0, t1;
     swap16(l, t0, t1);
     l = t0 + t1;
@@ -709,18 +848,20 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 1 : NB == 4 ? 2 : 3) void k_kv_atten
     float* o = sm + (wave * nh + col) * HD;
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i) {
-      // (the V tiles from high nibbles are 16 times their codes)
+      // (codes of high nibbles were 16 times themselves)
       const float f = KV == CHONK_KV_Q4 && (i & 1) ? 0.0625f : 1.f;
       *(float4*)(o + 16 * i + 4 * g) = make_float4(acc[i][0] * f, acc[i][1] * f, acc[i][2] * f, acc[i][3] * f);
     }
-    if (g == 0) {
-      ml[(wave * nh + col) * 2] = m;
-      ml[(wave * nh + col) * 2 + 1] = l;
-    }
+  }
+  if (PACK ? pc == 0 && hc < nh : g == 0 && col < nh) {
+    float* o = ml + (wave * nh + (PACK ? hc : col)) * 2;
+    o[0] = m;
+    o[1] = l;
   }
   __syncthreads();
-  float* prow = a.part + (int64_t)blockIdx.x * min(G, 16) * HD;
-  float* pml = a.part + (int64_t)kWantWgs * min(G, 16) * HD + (int64_t)blockIdx.x * min(G, 16) * 2;
+  const int nhm = min(G, 16);
+  float* prow = a.part + (int64_t)blockIdx.x * nhm * HD;
+  float* pml = a.part + (int64_t)a.want * nhm * HD + (int64_t)blockIdx.x * nhm * 2;
   for (int x = tid; x < nh * HD; x += kWg) {
     const int h = x / HD, d = x % HD;
     float M = -1e30f;
@@ -753,19 +894,18 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 1 : NB == 4 ? 2 : 3) void k_kv_atten
 // Joins a (row, head)'s segments: HD / 4 columns of float4, the segments over
 // groups of threads, every group's in order and the groups in order.
 __global__ __launch_bounds__(kWg) void k_kv_join(KvAttendArgs a) {
-  __shared__ int tmp[4], pick[3];
-  __shared__ float wt[kWantWgs];
+  __shared__ float wt[kMostWgs];
   __shared__ float red[8];
   __shared__ __align__(16) float so[kWg * 4];
   const int G = a.heads / a.c.kv_heads, hgs = (G + 15) / 16, items = a.c.kv_heads * hgs, nhm = min(G, 16);
   const int h = blockIdx.x, r = blockIdx.y, hd = a.c.hd, tid = threadIdx.x;
-  cut_rows(a, items, tmp, pick, [&](int t, int, int) { return t == r; });
-  const int segs = pick[2];
-  if (segs == 1) return;
+  const Cut cut = cut_rows(a, items, [&](int t, int, int) { return t == r; });
+  const int segs = cut.segs;
+  if (segs == 1 || cut.seq < 0) return;
   const int it = h / G * hgs + h % G / 16, hh = h % G % 16;
-  const int slot0 = pick[1] * items + it * segs;
+  const int slot0 = cut.before * items + it * segs;
   const float* rows = a.part + ((int64_t)slot0 * nhm + hh) * hd;
-  const float* ml = a.part + (int64_t)kWantWgs * nhm * hd + ((int64_t)slot0 * nhm + hh) * 2;
+  const float* ml = a.part + (int64_t)a.want * nhm * hd + ((int64_t)slot0 * nhm + hh) * 2;
   float M = -1e30f;
   for (int s = tid; s < segs; s += kWg) M = fmaxf(M, ml[(int64_t)s * nhm * 2]);
   M = wave_max(M);
@@ -804,9 +944,11 @@ __global__ __launch_bounds__(kWg) void k_kv_join(KvAttendArgs a) {
   }
 }
 
+// Segments wanted: as many workgroups as the registers let the 256 CUs hold at once.
+int attend_want(const KvCache& c) { return c.hd >= 256 ? 512 : c.hd == 128 ? 768 : 1024; }
 bool attend_splits(const KvCache& c, int rows, int heads) {
   const int64_t n = (int64_t)rows * c.kv_heads * ((heads / c.kv_heads + 15) / 16);
-  return rows <= kWg && n <= kWantWgs / 2 && 2 * c.max_pages > kMinHalves;
+  return rows <= 256 && n <= attend_want(c) / 2 && c.max_pages > kMinHalves;
 }
 
 }  // namespace
@@ -850,38 +992,35 @@ hipError_t launch_kv_read(const KvReadArgs& a, hipStream_t s) {
 }
 
 int64_t kv_attend_floats(const KvCache& c, int rows, int heads) {
-  return attend_splits(c, rows, heads) ? (int64_t)kWantWgs * std::min(heads / c.kv_heads, 16) * (c.hd + 2) : 0;
+  return attend_splits(c, rows, heads) ? (int64_t)attend_want(c) * std::min(heads / c.kv_heads, 16) * (c.hd + 2) : 0;
 }
 
 hipError_t launch_kv_attend(const KvAttendArgs& a0, hipStream_t s) {
   KvAttendArgs a = a0;
   const int G = a.heads / a.c.kv_heads, hgs = (G + 15) / 16, nh = std::min(G, 16);
   a.split = attend_splits(a.c, a.rows, a.heads) ? 1 : 0;
+  a.want = attend_want(a.c);
   if (a.split && !a.part) return hipErrorInvalidValue;
-  const dim3 grid(a.split ? kWantWgs : (uint32_t)((int64_t)a.rows * a.c.kv_heads * hgs));
+  const dim3 grid(a.split ? a.want : (uint32_t)((int64_t)a.rows * a.c.kv_heads * hgs));
   const size_t sh = (size_t)4 * nh * (a.c.hd + 2) * 4;
-#define CHONK_KV_CASE(T, B)                                                                              \
-  if (a.c.type == T && a.c.hd == 32 * B) {                                                               \
-    if (sh > 65536) {                                                                                    \
-      const hipError_t e = hipFuncSetAttribute((const void*)k_kv_attend<T, B>,                           \
+#define CHONK_KV_CASE(T, B, P)                                                                           \
+  if (a.c.type == T && a.c.hd == 32 * B && P == (nh <= 4)) {                                             \
+    if (sh > 32768) {                                                                                    \
+      const hipError_t e = hipFuncSetAttribute((const void*)k_kv_attend<T, B, P>,                        \
                                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)sh);     \
       if (e != hipSuccess) return e;                                                                     \
     }                                                                                                    \
-    hipLaunchKernelGGL((k_kv_attend<T, B>), grid, dim3(kWg), sh, s, a);                                  \
+    hipLaunchKernelGGL((k_kv_attend<T, B, P>), grid, dim3(kWg), sh, s, a);                               \
   } else
-  CHONK_KV_CASE(CHONK_KV_F16, 1)
-  CHONK_KV_CASE(CHONK_KV_F16, 2)
-  CHONK_KV_CASE(CHONK_KV_F16, 4)
-  CHONK_KV_CASE(CHONK_KV_F16, 8)
-  CHONK_KV_CASE(CHONK_KV_Q8, 1)
-  CHONK_KV_CASE(CHONK_KV_Q8, 2)
-  CHONK_KV_CASE(CHONK_KV_Q8, 4)
-  CHONK_KV_CASE(CHONK_KV_Q8, 8)
-  CHONK_KV_CASE(CHONK_KV_Q4, 1)
-  CHONK_KV_CASE(CHONK_KV_Q4, 2)
-  CHONK_KV_CASE(CHONK_KV_Q4, 4)
-  CHONK_KV_CASE(CHONK_KV_Q4, 8)
+#define CHONK_KV_CASES(T, P) CHONK_KV_CASE(T, 1, P) CHONK_KV_CASE(T, 2, P) CHONK_KV_CASE(T, 4, P) CHONK_KV_CASE(T, 8, P)
+  CHONK_KV_CASES(CHONK_KV_F16, false)
+  CHONK_KV_CASES(CHONK_KV_F16, true)
+  CHONK_KV_CASES(CHONK_KV_Q8, false)
+  CHONK_KV_CASES(CHONK_KV_Q8, true)
+  CHONK_KV_CASES(CHONK_KV_Q4, false)
+  CHONK_KV_CASES(CHONK_KV_Q4, true)
   return hipErrorInvalidValue;
+#undef CHONK_KV_CASES
 #undef CHONK_KV_CASE
   if (a.split) hipLaunchKernelGGL(k_kv_join, dim3(a.heads, a.rows), dim3(kWg), 0, s, a);
   return hipGetLastError();
