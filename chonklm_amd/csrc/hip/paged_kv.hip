@@ -63,26 +63,51 @@ __device__ __forceinline__ int place_of(int p) { return ((p & 15) >> 2) * 8 + (p
 
 // ---- writing ----------------------------------------------------------------------
 
+typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef _Float16 h4u_t __attribute__((ext_vector_type(4), aligned(2)));
+
+// Sums and maxima over the L lanes of a (row, head), without the LDS crossbar.
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int L>
+__device__ __forceinline__ double lanes_sum(double v) {
+  v += dpp64<0xb1>(v);
+  v += dpp64<0x4e>(v);
+  v += dpp64<0x141>(v);
+  if constexpr (L >= 16) v += dpp64<0x140>(v);
+  if constexpr (L >= 32) v += __shfl_xor(v, 16);
+  if constexpr (L >= 64) v += __shfl_xor(v, 32);
+  return v;
+}
+
 // Codes and scale of eight lanes' 32 values, four consecutive dims a lane. A
 // scale is the fp16 nearest to the exact one, and the codes count in units of
 // that fp16 number, so a code is off by at most half a unit of what is stored.
 template <int KV>
 __device__ __forceinline__ uint32_t quantise(const float (&y)[4], int (&c)[4]) {
   constexpr float kTop = KV == CHONK_KV_Q8 ? 127.f : 7.f, kLow = KV == CHONK_KV_Q8 ? -127.f : -8.f;
-  float m = 0.f;
-  int bad = 0;
+  // the largest magnitude; a NaN or an infinity makes it infinite
+  float m = y[0];
+  bool bad = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (fabsf(y[i]) > fabsf(m)) m = y[i];
     bad |= !(fabsf(y[i]) <= 3.402823466e38f);
   }
-#pragma unroll
-  for (int x = 1; x < 8; x *= 2) {
-    const float o = __shfl_xor(m, x);
-    bad |= __shfl_xor(bad, x);
-    // (of equal magnitudes the lower dim's: every lane must find the same one)
+  if (bad) m = INFINITY;
+  // (of equal magnitudes the lower dim's: every lane must find the same one)
+  auto step = [&](float o, int x) {
     if (fabsf(o) > fabsf(m) || (fabsf(o) == fabsf(m) && (threadIdx.x & x))) m = o;
-  }
+  };
+  step(dpp<0xb1>(m), 1);
+  step(dpp<0x4e>(m), 2);
+  step(dpp<0x141>(m), 4);  // (the other four's: a mirrored row of eight)
+  bad = fabsf(m) == INFINITY;
   float d = KV == CHONK_KV_Q8 ? __fdiv_rn(fabsf(m), 127.f) : m * -0.125f;
   d = fminf(fmaxf(d, -65504.f), 65504.f);
   const _Float16 h = (_Float16)d;
@@ -95,28 +120,27 @@ __device__ __forceinline__ uint32_t quantise(const float (&y)[4], int (&c)[4]) {
 
 // Four consecutive values of K (or V) at dims d0 .. d0 + 3 of position j of the
 // page into the head's part at `base`. The eight lanes of a block come together.
-template <int KV, bool IS_V>
-__device__ __forceinline__ void put4(uint8_t* base, int hd, int j, int d0, const float (&y)[4], bool ok) {
+template <int KV>
+__device__ __forceinline__ void put4(uint8_t* base, int hd, int j, int d0, const float (&y)[4], bool is_v, bool ok) {
   const int nb = hd / 32, b = d0 / 32, u = j / 32, p = j & 31, i0 = d0 & 31;
-  const int unit = u * nb + b;
+  const int unit = u * nb + b, pl = place_of(p);
+  // in a unit: K's run of eight dims (row p & 15, tile p >> 4), V's place of the first dim
+  const int nk = (i0 >> 3) * 16 + (p & 15), nv = (pl >> 3) * 16 + (i0 & 15);
   if constexpr (KV == CHONK_KV_F16) {
     _Float16* o = (_Float16*)base + (size_t)unit * 1024;
     h4_t v;
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = (_Float16)y[i];
     if (!ok) return;
-    if constexpr (!IS_V) {
-      *(h4_t*)(o + (p >> 4) * 512 + ((i0 >> 3) * 16 + (p & 15)) * 8 + (i0 & 7)) = v;
+    if (!is_v) {
+      *(h4_t*)(o + (p >> 4) * 512 + nk * 8 + (i0 & 7)) = v;
     } else {
-      const int pl = place_of(p);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        o[(i0 >> 4) * 512 + ((pl >> 3) * 16 + (i0 & 15) + i) * 8 + (pl & 7)] = v[i];
+      for (int i = 0; i < 4; ++i) o[(i0 >> 4) * 512 + (nv + i) * 8 + (pl & 7)] = v[i];
     }
   } else {
     int c[4];
     const uint32_t d = quantise<KV>(y, c);
-    const int pl = place_of(p);
     uint16_t* sc = (uint16_t*)(base + kv_code_bytes(KV, hd));
     if (ok && i0 == 0) sc[unit * 32 + pl] = (uint16_t)d;
     if constexpr (KV == CHONK_KV_Q8) {
@@ -124,31 +148,27 @@ __device__ __forceinline__ void put4(uint8_t* base, int hd, int j, int d0, const
 #pragma unroll
       for (int i = 0; i < 4; ++i) c[i] += 128;
       if (!ok) return;
-      if constexpr (!IS_V) {
-        *(uint32_t*)(o + ((i0 >> 3) * 16 + (p & 15)) * 16 + (p >> 4) * 8 + (i0 & 7)) =
-            (uint32_t)(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24);
+      if (!is_v) {
+        *(uint32_t*)(o + nk * 16 + (p >> 4) * 8 + (i0 & 7)) = (uint32_t)(c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24);
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          o[((pl >> 3) * 16 + (i0 & 15) + i) * 16 + (i0 >> 4) * 8 + (pl & 7)] = (uint8_t)c[i];
+        for (int i = 0; i < 4; ++i) o[(nv + i) * 16 + (i0 >> 4) * 8 + (pl & 7)] = (uint8_t)c[i];
       }
     } else {
       uint8_t* o = base + (size_t)unit * 512;
       // the lane with the other nibbles: dims + 4 (K), dims + 16 (V)
-      constexpr int X = IS_V ? 4 : 1;
       int n[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         c[i] += 8;
-        n[i] = c[i] | __shfl_xor(c[i], X) << 4;
+        n[i] = c[i] | (is_v ? __shfl_xor(c[i], 4) : __shfl_xor(c[i], 1)) << 4;
       }
-      if (!ok || (threadIdx.x & X)) return;
-      if constexpr (!IS_V) {
-        *(uint32_t*)(o + ((i0 >> 3) * 16 + (p & 15)) * 8 + (p >> 4) * 4) =
-            (uint32_t)(n[0] | n[1] << 8 | n[2] << 16 | n[3] << 24);
+      if (!ok || (threadIdx.x & (is_v ? 4 : 1))) return;
+      if (!is_v) {
+        *(uint32_t*)(o + nk * 8 + (p >> 4) * 4) = (uint32_t)(n[0] | n[1] << 8 | n[2] << 16 | n[3] << 24);
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[((pl >> 3) * 16 + (i0 & 15) + i) * 8 + (pl & 7)] = (uint8_t)n[i];
+        for (int i = 0; i < 4; ++i) o[(nv + i) * 8 + (pl & 7)] = (uint8_t)n[i];
       }
     }
   }
@@ -158,104 +178,122 @@ __device__ __forceinline__ void put4(uint8_t* base, int hd, int j, int d0, const
 template <bool F16>
 __device__ __forceinline__ void row4(const PartSum& P, const _Float16* p16, int64_t ld, int r, int col, float (&v)[4]) {
   if constexpr (F16) {
-    const _Float16* p = p16 + r * ld + col;
+    const h4u_t x = *(const h4u_t*)(p16 + r * ld + col);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = (float)p[i];
+    for (int i = 0; i < 4; ++i) v[i] = (float)x[i];
   } else {
-    const int j[4] = {col, col + 1, col + 2, col + 3};
-    part_gather<4>(P, r, j, v);
+    const float* p = P.p + r * ld + col;
+    const f4u_t x = *(const f4u_t*)p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = x[i];
+    for (int z = 1; z < P.ks; ++z) {
+      const f4u_t w = *(const f4u_t*)(p + z * P.zs);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += w[i];
+    }
   }
 }
 
-// One wave per (row, head): q heads, then kv heads (K and V). Lane t holds dims
-// 4 t .. 4 t + 3, so a block of 32 is eight lanes. Every product and sum after
-// the norm's is rounded by itself (no fused multiply-add) and the norm's sum of squares is taken in 64
-// bits: the codes do not depend on which path (prompt rows or single tokens)
-// wrote them.
-template <int KV, bool F16>
+// A (row, q head), (row, kv head of K) or (row, kv head of V) takes 8 NB lanes,
+// four dims a lane; consecutive groups of lanes are consecutive rows of one head,
+// whose codes lie together. Everything that does not hang on the row's place is
+// asked for at once with it: a wave's time is three trips to memory (place, then
+// page and angles, then the stores), not one for each thing it needs.
+// Every product and sum after the norm's is rounded by itself (no fused multiply-add)
+// and the norm's sum of squares is taken in 64 bits: the codes do not depend on which
+// path (prompt rows or single tokens) wrote them.
+template <int KV, bool F16, int NB>
 __global__ __launch_bounds__(kWg) void k_kv_append(KvAppendArgs a) {
 #pragma clang fp contract(off)
-  __shared__ float xs[4][256];
-  const int r = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int hh = blockIdx.y * 4 + wave, qh = (F16 ? a.q16 != nullptr : a.q.p != nullptr) ? a.heads : 0;
-  if (hh >= qh + a.c.kv_heads) return;
+  constexpr int L = 8 * NB, HD = 32 * NB;
+  __shared__ __align__(16) float xs[kWg * 4];
+  const int tid = threadIdx.x, d0 = (tid & (L - 1)) * 4;
+  const int qh = (F16 ? a.q16 != nullptr : a.q.p != nullptr) ? a.heads : 0, kvh = a.c.kv_heads;
+  const uint32_t task = blockIdx.x * (kWg / L) + tid / L, tasks = (uint32_t)a.rows * (qh + 2 * kvh);
+  const bool in = task < tasks;
+  const uint32_t slot = min(task, tasks - 1) / (uint32_t)a.rows;
+  const int r = (int)(min(task, tasks - 1) - slot * (uint32_t)a.rows);
+  const bool is_q = (int)slot < qh, is_v = (int)slot >= qh + kvh;
+  const int h = is_q ? slot : is_v ? slot - qh - kvh : slot - qh;
   const int seq = a.at.seq ? a.at.seq[r] : a.at.seq0, pos = a.at.pos ? a.at.pos[r] : a.at.p0 + r;
-  if (seq < 0) return;
-  const int hd = a.c.hd, d0 = 4 * lane;
-  const bool ok = d0 < hd, is_k = hh >= qh;
-  const int kv = hh - qh;
-  const int page = page_of(a.c, seq, pos, lane == 0);
-  if (page < 0) return;
-  if (a.rope && pos >= a.rope_n) {
-    if (lane == 0) fault(a.c, KVF_POS);
-    return;
+  float y[4];
+  row4<F16>(is_q ? a.q : is_v ? a.v : a.k, is_q ? a.q16 : is_v ? a.v16 : a.k16, is_q ? a.q_ld : is_v ? a.v_ld : a.k_ld, r,
+            h * HD + d0, y);
+  const float* w = is_q ? a.qn_w : is_v ? nullptr : a.kn_w;
+  float4 wt = make_float4(1.f, 1.f, 1.f, 1.f);
+  if (w) wt = make_float4(w[d0], w[d0 + 1], w[d0 + 2], w[d0 + 3]);
+  // where the row goes; one that names no place goes nowhere
+  int page = 0;
+  bool ok = in && seq >= 0;
+  if (ok) {
+    page = page_of(a.c, seq, pos, d0 == 0);
+    ok = page >= 0;
+    if (ok && a.rope && pos >= a.rope_n) {
+      if (d0 == 0) fault(a.c, KVF_POS);
+      ok = false;
+    }
   }
-  float y[4] = {0.f, 0.f, 0.f, 0.f};
-  if (ok) row4<F16>(is_k ? a.k : a.q, is_k ? a.k16 : a.q16, is_k ? a.k_ld : a.q_ld, r, (is_k ? kv : hh) * hd + d0, y);
-  const float* w = is_k ? a.kn_w : a.qn_w;
   if (w) {
-    double ss = 0.0;
+    double sq = 0.0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ss += (double)y[i] * (double)y[i];
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) ss += __shfl_xor(ss, x);
-    const float inv = (float)(1.0 / sqrt(ss / hd + a.eps));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = ok ? y[i] * inv * w[d0 + i] : 0.f;
+    for (int i = 0; i < 4; ++i) sq += (double)y[i] * (double)y[i];
+    sq = lanes_sum<L>(sq);
+    const float inv = (float)(1.0 / sqrt(sq / HD + a.eps));
+    y[0] = y[0] * inv * wt.x;
+    y[1] = y[1] * inv * wt.y;
+    y[2] = y[2] * inv * wt.z;
+    y[3] = y[3] * inv * wt.w;
   }
-  if (a.rope) {
-    float* x = xs[wave];
-    if (ok) *(float4*)(x + d0) = make_float4(y[0], y[1], y[2], y[3]);
+  if (a.rope && !a.interleaved) {  // the other half's dims are other lanes'
+    *(float4*)(xs + 4 * tid) = make_float4(y[0], y[1], y[2], y[3]);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+  }
+  if (a.rope && !is_v && ok) {
     const int half = a.rope_dim / 2;
     const float2* cs = a.rope + (size_t)pos * half;
+    if (a.interleaved) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = d0 + i;
-      if (d >= a.rope_dim) continue;
-      const int pair = a.interleaved ? d >> 1 : d < half ? d : d - half;
-      const bool second = a.interleaved ? (d & 1) != 0 : d >= half;
-      const float2 t = cs[pair];
-      const float u = x[a.interleaved ? 2 * pair : pair], v = x[a.interleaved ? 2 * pair + 1 : pair + half];
-      y[i] = second ? u * t.y + v * t.x : u * t.x - v * t.y;
+      for (int i = 0; i < 4; i += 2) {
+        if (d0 + i >= a.rope_dim) continue;
+        const float2 t = cs[(d0 + i) / 2];
+        const float u = y[i], v = y[i + 1];
+        y[i] = u * t.x - v * t.y;
+        y[i + 1] = u * t.y + v * t.x;
+      }
+    } else {
+      const float* x = xs + 4 * tid - d0;  // the head's dims
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = d0 + i;
+        if (d >= a.rope_dim) continue;
+        const bool second = d >= half;
+        const float2 t = cs[second ? d - half : d];
+        const float o = x[second ? d - half : d + half];
+        y[i] = second ? o * t.y + y[i] * t.x : y[i] * t.x - o * t.y;
+      }
     }
   }
-  if (!is_k) {
+  if (is_q) {
     if (!ok) return;
-    const int64_t o = r * a.qo_ld + hh * hd + d0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (F16)
-        ((_Float16*)a.q_out)[o + i] = (_Float16)y[i];
-      else
-        ((float*)a.q_out)[o + i] = y[i];
-    }
+    const int64_t o = r * a.qo_ld + h * HD + d0;
+    if constexpr (F16)
+      *(h4u_t*)((_Float16*)a.q_out + o) = h4u_t{(_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
+    else
+      *(f4u_t*)((float*)a.q_out + o) = f4u_t{y[0], y[1], y[2], y[3]};
     return;
   }
-  const int part = kv_part_bytes(KV, hd), j = pos & (kKvPage - 1);
-  uint8_t* base = a.c.pages + ((size_t)page * a.c.kv_heads + kv) * 2 * part;
-  put4<KV, false>(base, hd, j, d0, y, ok);
-  if (ok)
-    row4<F16>(a.v, a.v16, a.v_ld, r, kv * hd + d0, y);
-  else
-    y[0] = y[1] = y[2] = y[3] = 0.f;
-  put4<KV, true>(base + part, hd, j, d0, y, ok);
+  constexpr int PART = kv_part_bytes(KV, HD);
+  uint8_t* base = a.c.pages + (((size_t)(ok ? page : 0) * kvh + h) * 2 + (is_v ? 1 : 0)) * PART;
+  put4<KV>(base, HD, pos & (kKvPage - 1), d0, y, is_v, ok);
 }
 
 // ---- reading back -----------------------------------------------------------------
 
-// One thread per (row, kv head, eight dims).
+// One thread per (row, kv head, eight dims): rows anywhere.
 template <int KV, bool F16>
-__global__ __launch_bounds__(kWg) void k_kv_read(KvReadArgs a) {
-  const int hd = a.c.hd, runs = hd / 8;
-  const int64_t id = (int64_t)blockIdx.x * kWg + threadIdx.x;
-  const int64_t rk = id / runs;
-  const int d0 = (int)(id % runs) * 8, kv = (int)(rk % a.c.kv_heads);
-  const int64_t r = rk / a.c.kv_heads;
-  if (r >= a.rows) return;
-  const int seq = a.at.seq ? a.at.seq[r] : a.at.seq0, pos = a.at.pos ? a.at.pos[r] : a.at.p0 + (int)r;
-  if (seq < 0) return;
+__device__ __forceinline__ void read8(const KvReadArgs& a, int r, int kv, int d0, int seq, int pos) {
+  const int hd = a.c.hd;
   const int page = page_of(a.c, seq, pos, d0 == 0);
   if (page < 0) return;
   const int part = kv_part_bytes(KV, hd), j = pos & (kKvPage - 1), p = j & 31, pl = place_of(p);
@@ -292,12 +330,142 @@ __global__ __launch_bounds__(kWg) void k_kv_read(KvReadArgs a) {
         x[i] = (float)c * d;
       }
     }
+    if constexpr (F16) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (F16)
-        ((_Float16*)out)[o + i] = (_Float16)x[i];
-      else
-        ((float*)out)[o + i] = x[i];
+      for (int i = 0; i < 8; i += 4)
+        *(h4u_t*)((_Float16*)out + o + i) = h4u_t{(_Float16)x[i], (_Float16)x[i + 1], (_Float16)x[i + 2], (_Float16)x[i + 3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) *(f4u_t*)((float*)out + o + i) = f4u_t{x[i], x[i + 1], x[i + 2], x[i + 3]};
+    }
+  }
+}
+
+// Byte (or nibble pair) k of a piece's words.
+__device__ __forceinline__ int byte_of(uint32_t w, int k) { return (int)(w >> (8 * k) & 0xff); }
+
+// A wave per (32 rows, kv head, block of 32 dims). Rows that are a half page's
+// positions (what a prompt's and a history's are, but at its ends) are read in the pages' own
+// order, a unit of 1 KiB (8 bits) at a time, and leave in whole 64-byte pieces; others
+// one by one. The rows' groups start where row 0's half page does.
+template <int KV, bool F16>
+__global__ __launch_bounds__(kWg) void k_kv_read(KvReadArgs a) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hd = a.c.hd, nb = hd / 32;
+  const int shift = (a.at.pos ? a.at.pos[0] : a.at.p0) & 31;
+  const int groups = (a.rows + shift + 31) / 32;
+  // (kv heads and blocks before rows: a row's pieces are written close in time)
+  const int64_t task = (int64_t)blockIdx.x * 4 + wave;
+  const int per = a.c.kv_heads * nb;
+  const int grp = (int)(task / per), it = (int)(task % per), kv = it / nb, b = it % nb;
+  if (grp >= groups) return;
+  const int r0 = grp * 32 - shift, r = r0 + (lane & 31);
+  const bool in = r >= 0 && r < a.rows;
+  const int rc = min(max(r, 0), a.rows - 1);
+  const int seq = a.at.seq ? a.at.seq[rc] : a.at.seq0, pos = a.at.pos ? a.at.pos[rc] : a.at.p0 + rc;
+  // the half page that the first of the group's rows would make it
+  const int first = __builtin_ctzll(__ballot(in));
+  const int s0 = __builtin_amdgcn_readlane(seq, first), p0 = __builtin_amdgcn_readlane(pos, first) - first;
+  const bool odd = in && (seq != s0 || pos != p0 + (lane & 31));
+  if (__ballot(odd) || (p0 & 31) || p0 < 0 || s0 < 0) {
+    // four lanes a row: its eight-dim runs of this block
+    for (int i = 0; i < 2; ++i) {
+      const int rr = r0 + 16 * i + (lane >> 2);
+      if (rr < 0 || rr >= a.rows) continue;
+      const int s = a.at.seq ? a.at.seq[rr] : a.at.seq0, p = a.at.pos ? a.at.pos[rr] : a.at.p0 + rr;
+      if (s >= 0) read8<KV, F16>(a, rr, kv, 32 * b + 8 * (lane & 3), s, p);
+    }
+    return;
+  }
+  const int page = page_of(a.c, s0, p0, lane == 0);
+  if (page < 0) return;
+  const int part = kv_part_bytes(KV, hd), u = p0 / 32 & 1, unit = u * nb + b, g = lane >> 4, i = lane & 15;
+  const uint8_t* base = a.c.pages + ((size_t)page * a.c.kv_heads + kv) * 2 * part;
+  const int64_t o = r0 * a.row_ld + kv * a.head_ld + 32 * b;  // (of the group's row 0, which may lie before the first)
+  constexpr int W = KV == CHONK_KV_F16 ? 8 : KV == CHONK_KV_Q8 ? 4 : 2;
+  uint32_t w[2][W];
+  uint4 dk[2];
+  uint32_t ds[2];
+#pragma unroll
+  for (int v = 0; v < 2; ++v) {
+    const uint8_t* src = base + v * part + (size_t)unit * (256 * W);
+    if constexpr (KV == CHONK_KV_Q4) {
+      const uint2 x = ldg2(src + lane * 8);
+      w[v][0] = x.x, w[v][1] = x.y;
+    } else {
+#pragma unroll
+      for (int t = 0; t < W / 4; ++t) {
+        const uint4 x = ldg4(src + t * 1024 + lane * 16);
+        w[v][4 * t] = x.x, w[v][4 * t + 1] = x.y, w[v][4 * t + 2] = x.z, w[v][4 * t + 3] = x.w;
+      }
+    }
+    if constexpr (KV != CHONK_KV_F16) {
+      const uint8_t* s = base + v * part + kv_code_bytes(KV, hd) + unit * 64;
+      if (v) {
+        dk[1] = ldg4(s + g * 16);  // V: of the lane's eight positions
+      } else {                     // K: of positions i and 16 + i
+        ds[0] = ((const uint16_t*)s)[place_of(i)];
+        ds[1] = ((const uint16_t*)s)[place_of(16 + i)];
+      }
+    }
+  }
+  if (a.k) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (KV == CHONK_KV_F16)
+          x[e] = h2f(w[0][4 * t + e / 2] >> (16 * (e & 1)));
+        else if constexpr (KV == CHONK_KV_Q8)
+          x[e] = (float)(byte_of(w[0][2 * t + e / 4], e & 3) - 128) * h2f(ds[t]);
+        else
+          x[e] = (float)((int)(w[0][t] >> (8 * (e & 3) + 4 * (e >> 2)) & 15) - 8) * h2f(ds[t]);
+      }
+      const int rr = r0 + 16 * t + i;
+      if (rr < 0 || rr >= a.rows) continue;
+      const int64_t at = o + (16 * t + i) * a.row_ld + 8 * g;
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        if constexpr (F16)
+          *(h4u_t*)((_Float16*)a.k + at + e) =
+              h4u_t{(_Float16)x[e], (_Float16)x[e + 1], (_Float16)x[e + 2], (_Float16)x[e + 3]};
+        else
+          *(f4u_t*)((float*)a.k + at + e) = f4u_t{x[e], x[e + 1], x[e + 2], x[e + 3]};
+      }
+    }
+  }
+  if (a.v) {
+    const uint32_t dw[4] = {dk[1].x, dk[1].y, dk[1].z, dk[1].w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int j = 4 * g + (e & 3) + 16 * (e >> 2), rr = r0 + j;
+      const float d = KV == CHONK_KV_F16 ? 1.f : h2f(dw[e / 2] >> (16 * (e & 1)));
+      float x[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if constexpr (KV == CHONK_KV_F16)
+          x[h] = h2f(w[1][4 * h + e / 2] >> (16 * (e & 1)));
+        else if constexpr (KV == CHONK_KV_Q8)
+          x[h] = (float)(byte_of(w[1][2 * h + e / 4], e & 3) - 128) * d;
+        else
+          x[h] = (float)((int)(w[1][e / 4] >> (8 * (e & 3) + 4 * h) & 15) - 8) * d;
+      }
+      const int64_t at = o + j * a.row_ld + i;
+      if constexpr (F16) {
+        // neighbours trade halves, so that each stores two dims together: the even lane
+        // those of the block's first 16, the odd lane those of its last
+        const uint32_t mine = (uint32_t)__builtin_bit_cast(unsigned short, (_Float16)x[0]) |
+                              (uint32_t)__builtin_bit_cast(unsigned short, (_Float16)x[1]) << 16;
+        const uint32_t its = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)mine, 0xb1, 0xf, 0xf, false);
+        const uint32_t two = __builtin_amdgcn_perm(its, mine, i & 1 ? 0x03020706u : 0x05040100u);
+        if (rr < 0 || rr >= a.rows) continue;
+        typedef uint32_t u1_t __attribute__((aligned(2)));
+        *(u1_t*)((_Float16*)a.v + at + (i & 1 ? 15 : 0)) = two;
+      } else {
+        if (rr < 0 || rr >= a.rows) continue;
+        ((float*)a.v)[at] = x[0];
+        ((float*)a.v)[at + 16] = x[1];
+      }
     }
   }
 }
@@ -311,8 +479,8 @@ __global__ __launch_bounds__(kWg) void k_kv_read(KvReadArgs a) {
 // (0, 2, 1, 3, 4, 6, 5, 7): both products take their k in that order.
 // (As denormals, one operation for two codes, the matrix unit takes them too; but it
 // aligns such a product by the exponent 2^-14 that denormals share, and a code of b bits
-// loses 10 - b of the product's 24: results were off by 1e-5 with 4 bits, and by
-// 2.5e-6 instead of 5e-7 with 8, for 4 us of 22 at 41k positions.)
+// loses 10 - b of the product's 24: results were off by 1e-5 with 4 bits and by
+// 2.5e-6 instead of 9e-7 with 8, and no call was faster.)
 __device__ __forceinline__ uint32_t less2(uint32_t v, uint32_t k) {
   return __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2_t, v) - __builtin_bit_cast(h2_t, k));
 }
@@ -954,27 +1122,30 @@ bool attend_splits(const KvCache& c, int rows, int heads) {
 }  // namespace
 
 hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t s) {
-  const int nh = ((a.f16 ? a.q16 != nullptr : a.q.p != nullptr) ? a.heads : 0) + a.c.kv_heads;
-  const dim3 grid(a.rows, (nh + 3) / 4);
-#define CHONK_KV_CASE(T)                                                                \
-  case T:                                                                               \
-    if (a.f16)                                                                          \
-      hipLaunchKernelGGL((k_kv_append<T, true>), grid, dim3(kWg), 0, s, a);             \
-    else                                                                                \
-      hipLaunchKernelGGL((k_kv_append<T, false>), grid, dim3(kWg), 0, s, a);            \
-    return hipGetLastError();
-  switch (a.c.type) {
-    CHONK_KV_CASE(CHONK_KV_F16)
-    CHONK_KV_CASE(CHONK_KV_Q8)
-    CHONK_KV_CASE(CHONK_KV_Q4)
-    default: return hipErrorInvalidValue;
-  }
+  const int slots = ((a.f16 ? a.q16 != nullptr : a.q.p != nullptr) ? a.heads : 0) + 2 * a.c.kv_heads;
+  const int per = kWg / (a.c.hd / 4);
+  const dim3 grid((uint32_t)(((int64_t)a.rows * slots + per - 1) / per));
+#define CHONK_KV_CASE(T, B)                                                                 \
+  if (a.c.type == T && a.c.hd == 32 * B) {                                                  \
+    if (a.f16)                                                                              \
+      hipLaunchKernelGGL((k_kv_append<T, true, B>), grid, dim3(kWg), 0, s, a);              \
+    else                                                                                    \
+      hipLaunchKernelGGL((k_kv_append<T, false, B>), grid, dim3(kWg), 0, s, a);             \
+  } else
+#define CHONK_KV_CASES(T) CHONK_KV_CASE(T, 1) CHONK_KV_CASE(T, 2) CHONK_KV_CASE(T, 4) CHONK_KV_CASE(T, 8)
+  CHONK_KV_CASES(CHONK_KV_F16)
+  CHONK_KV_CASES(CHONK_KV_Q8)
+  CHONK_KV_CASES(CHONK_KV_Q4)
+  return hipErrorInvalidValue;
+#undef CHONK_KV_CASES
 #undef CHONK_KV_CASE
+  return hipGetLastError();
 }
 
 hipError_t launch_kv_read(const KvReadArgs& a, hipStream_t s) {
-  const int64_t n = (int64_t)a.rows * a.c.kv_heads * (a.c.hd / 8);
-  const dim3 grid((uint32_t)((n + kWg - 1) / kWg));
+  // (one group more than the rows fill: where the first half page starts is the device's to know)
+  const int64_t waves = ((int64_t)a.rows + 31 + 31) / 32 * a.c.kv_heads * (a.c.hd / 32);
+  const dim3 grid((uint32_t)((waves + 3) / 4));
 #define CHONK_KV_CASE(T)                                                                \
   case T:                                                                               \
     if (a.f16)                                                                          \
@@ -1136,7 +1307,7 @@ int chonk_kv_append(const chonk_kv_cache* cache, const chonk_kv_rows* rows, cons
     if (x->k_norm || x->q_norm) {
       if (!(x->eps >= 0.0)) throw Error(CHONK_EINVAL, "paged K/V cache: eps must not be negative");
     }
-    check_grid((int64_t)rows->n * ((x->q ? x->heads : 0) + a.c.kv_heads + 3) / 4);
+    check_grid((int64_t)rows->n * ((x->q ? x->heads : 0) + 2 * a.c.kv_heads) * (a.c.hd / 4) / kWg);
     a.at.seq = rows->seq;
     a.at.pos = rows->pos;
     a.rows = rows->n;
@@ -1189,7 +1360,7 @@ int chonk_kv_read(const chonk_kv_cache* cache, const chonk_kv_rows* rows, int32_
     const bool rows_out = head_stride >= hd && row_stride >= (a.c.kv_heads - 1) * head_stride + hd;
     const bool heads_out = row_stride >= hd && head_stride >= (int64_t)(rows->n - 1) * row_stride + hd;
     if (!rows_out && !heads_out) throw Error(CHONK_EINVAL, "paged K/V cache: result rows overlap");
-    check_grid((int64_t)rows->n * a.c.kv_heads * (a.c.hd / 8) / kWg);
+    check_grid(((int64_t)rows->n / 32 + 2) * a.c.kv_heads * (a.c.hd / 32) / 4);
     a.at.seq = rows->seq;
     a.at.pos = rows->pos;
     a.rows = rows->n;

@@ -17,6 +17,7 @@ libchonk.so then runs on torch's HIP runtime, whose pointers and streams it is g
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import sys
 from typing import Optional
 
@@ -38,6 +39,12 @@ def _refuse(message: str):
     raise ChonkError(CHONK_EINVAL, "paged K/V cache: " + message)
 
 
+# torch's current stream of a device, as a hipStream_t (what torch.cuda.current_stream().cuda_stream says)
+_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    lambda at: torch.cuda.current_stream(at).cuda_stream
+
+
+@functools.lru_cache(maxsize=None)
 def page_bytes(kv_dtype: str, kv_heads: int, head_dim: int) -> int:
     """Bytes of one page (64 positions of K and V of every kv head)."""
     if kv_dtype not in KV_TYPES:
@@ -69,47 +76,52 @@ class PagedKv:
         if _OWN_RUNTIME:
             _refuse("libchonk.so was loaded before torch and uses another HIP runtime: import torch first")
         size = page_bytes(kv_dtype, kv_heads, head_dim)
-        if pages.dtype != torch.uint8 or pages.dim() != 2 or pages.shape[1] != size or not pages.is_contiguous():
+        shape, tshape = pages.shape, table.shape
+        if pages.dtype != torch.uint8 or len(shape) != 2 or shape[1] != size or not pages.is_contiguous():
             _refuse(f"pages must be contiguous uint8 [n_pages, {size}]")
-        if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
+        if table.dtype != torch.int32 or len(tshape) != 2 or not table.is_contiguous():
             _refuse("table must be contiguous int32 [n_seqs, max_pages]")
         if not pages.is_cuda:
             _refuse("pages must be on a GPU")
-        if table.device != pages.device or (fault is not None and fault.device != pages.device):
+        at = pages.get_device()
+        if table.get_device() != at or (fault is not None and fault.get_device() != at):
             _refuse("table and fault must be on the pages' device")
         if fault is not None and (fault.dtype != torch.int32 or fault.numel() != 1):
             _refuse("fault must be int32 [1]")
         self.pages, self.table, self.fault = pages, table, fault
-        self.kv_heads, self.head_dim, self.device = kv_heads, head_dim, pages.device
-        self._c = _lib.KvCacheC(KV_TYPES[kv_dtype], kv_heads, head_dim, pages.shape[0], pages.data_ptr(),
-                                table.shape[0], table.shape[1], table.data_ptr(),
-                                fault.data_ptr() if fault is not None else None, pages.device.index)
+        self.kv_heads, self.head_dim, self._at = kv_heads, head_dim, at
+        self._c = C.byref(_lib.KvCacheC(KV_TYPES[kv_dtype], kv_heads, head_dim, shape[0], pages.data_ptr(), tshape[0],
+                                        tshape[1], table.data_ptr(), fault.data_ptr() if fault is not None else None, at))
+
+    @property
+    def device(self) -> torch.device:
+        return self.pages.device
 
     # -- arguments ------------------------------------------------------------------
-    def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
+    def _index(self, x: torch.Tensor, n: int, name: str) -> int:
+        if x.dtype != torch.int32 or x.shape != (n,) or x.get_device() != self._at or not x.is_contiguous():
+            _refuse(f"{name} must be contiguous int32 [{n}] on {self.device}")
+        return x.data_ptr()
 
-    def _index(self, x: torch.Tensor, n: int, name: str) -> torch.Tensor:
-        if x.dtype != torch.int32 or x.dim() != 1 or x.shape[0] != n or x.device != self.device:
-            _refuse(f"{name} must be int32 [{n}] on {self.device}")
-        return x if x.is_contiguous() else x.contiguous()
-
-    def _rows(self, x: torch.Tensor, heads: Optional[int], dtype: Optional[torch.dtype], name: str) -> int:
+    def _rows(self, x: torch.Tensor, n: int, heads: int, dtype: torch.dtype, name: str) -> int:
         """Checks rows [n, heads, head_dim] and returns the elements from row to row."""
-        if x.dim() != 3 or x.shape[2] != self.head_dim or (heads is not None and x.shape[1] != heads):
-            _refuse(f"{name} must be [n, {heads if heads is not None else 'heads'}, {self.head_dim}]")
-        if x.dtype not in _ACT or (dtype is not None and x.dtype != dtype):
-            _refuse(f"{name} must be {dtype or 'float32 or float16'}")
-        if x.device != self.device:
+        if x.shape != (n, heads, self.head_dim):
+            _refuse(f"{name} must be [{n}, {heads}, {self.head_dim}]")
+        if x.dtype != dtype:
+            _refuse(f"{name} must be {dtype}")
+        if x.get_device() != self._at:
             _refuse(f"{name} must be on {self.device}")
-        if (x.stride(2) != 1 or (x.shape[1] > 1 and x.stride(1) != self.head_dim)) and x.numel():
+        row, head, one = x.stride()
+        if n == 0:
+            return heads * self.head_dim
+        if one != 1 or (heads > 1 and head != self.head_dim):
             _refuse(f"a row of {name} must be contiguous")
-        return x.stride(0) if x.shape[0] > 1 else x.shape[1] * self.head_dim
+        return row if n > 1 else heads * self.head_dim
 
     def _weights(self, x: Optional[torch.Tensor], name: str) -> Optional[int]:
         if x is None:
             return None
-        if x.dtype != torch.float32 or x.shape != (self.head_dim,) or x.device != self.device or not x.is_contiguous():
+        if x.dtype != torch.float32 or x.shape != (self.head_dim,) or x.get_device() != self._at or not x.is_contiguous():
             _refuse(f"{name} must be contiguous float32 [{self.head_dim}] on {self.device}")
         return x.data_ptr()
 
@@ -122,44 +134,51 @@ class PagedKv:
         [n, heads, head_dim] (None without q), q and k normalised per head and rotated where the
         weights and the table [positions, rope_dim / 2, 2] are given. `out` may be q.
         Rows with a negative sequence are left out."""
-        n = k.shape[0]
-        k_ld = self._rows(k, self.kv_heads, None, "k")
-        v_ld = self._rows(v, self.kv_heads, k.dtype, "v")
-        if v.shape[0] != n:
-            _refuse("k and v differ in rows")
-        q_ld = o_ld = heads = 0
+        dtype, n = k.dtype, len(k)
+        if dtype not in _ACT:
+            _refuse("k must be float32 or float16")
+        k_ld = self._rows(k, n, self.kv_heads, dtype, "k")
+        v_ld = self._rows(v, n, self.kv_heads, dtype, "v")
+        q_at = out_at = rope_at = None
+        q_ld = o_ld = heads = rope_dim = rope_n = 0
         if q is not None:
-            q_ld, heads = self._rows(q, None, k.dtype, "q"), q.shape[1]
+            if q.dim() != 3:
+                _refuse("q must be [n, heads, head_dim]")
+            heads = q.shape[1]
+            q_ld = self._rows(q, n, heads, dtype, "q")
             if out is None:
-                out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-            o_ld = self._rows(out, heads, k.dtype, "out")
-            if q.shape[0] != n or out.shape[0] != n:
-                _refuse("q, k and out differ in rows")
+                out, o_ld = torch.empty_like(q, memory_format=torch.contiguous_format), heads * self.head_dim
+            else:
+                o_ld = self._rows(out, n, heads, dtype, "out")
+            q_at, out_at = q.data_ptr(), out.data_ptr()
         elif out is not None:
             _refuse("out without q")
-        if rope is not None and (rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[2] != 2 or
-                                 not rope.is_contiguous() or rope.device != self.device):
-            _refuse(f"rope must be contiguous float32 [positions, rope_dim / 2, 2] on {self.device}")
-        seqs, positions = self._index(seqs, n, "seqs"), self._index(positions, n, "positions")
-        rows = _lib.KvRowsC(n, seqs.data_ptr(), positions.data_ptr())
-        a = _lib.KvAppendArgsC(
-            _ACT[k.dtype], heads, q.data_ptr() if q is not None else None, k.data_ptr(), v.data_ptr(),
-            out.data_ptr() if out is not None else None, q_ld, k_ld, v_ld, o_ld, self._weights(q_norm, "q_norm"),
-            self._weights(k_norm, "k_norm"), eps, rope.data_ptr() if rope is not None else None,
-            2 * rope.shape[1] if rope is not None else 0, rope.shape[0] if rope is not None else 0, bool(interleaved))
-        check(lib().chonk_kv_append(C.byref(self._c), C.byref(rows), C.byref(a), self._stream()))
+        if rope is not None:
+            if (rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[2] != 2 or not rope.is_contiguous() or
+                    rope.get_device() != self._at):
+                _refuse(f"rope must be contiguous float32 [positions, rope_dim / 2, 2] on {self.device}")
+            rope_at, rope_n, rope_dim = rope.data_ptr(), rope.shape[0], 2 * rope.shape[1]
+        rows = _lib.KvRowsC(n, self._index(seqs, n, "seqs"), self._index(positions, n, "positions"))
+        a = _lib.KvAppendArgsC(_ACT[dtype], heads, q_at, k.data_ptr(), v.data_ptr(), out_at, q_ld, k_ld, v_ld, o_ld,
+                               self._weights(q_norm, "q_norm"), self._weights(k_norm, "k_norm"), eps, rope_at, rope_dim,
+                               rope_n, bool(interleaved))
+        status = lib().chonk_kv_append(self._c, C.byref(rows), C.byref(a), _stream(self._at))
+        if status:
+            check(status)
         return out
 
     def read(self, seqs: torch.Tensor, positions: torch.Tensor, dtype: torch.dtype = torch.float16):
         """The values stored at (seqs[i], positions[i]): k, v [n, kv_heads, head_dim]."""
         if dtype not in _ACT:
             _refuse("dtype must be float32 or float16")
-        n = seqs.shape[0]
-        seqs, positions = self._index(seqs, n, "seqs"), self._index(positions, n, "positions")
-        k, v = (torch.empty((n, self.kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2))
-        rows = _lib.KvRowsC(n, seqs.data_ptr(), positions.data_ptr())
-        check(lib().chonk_kv_read(C.byref(self._c), C.byref(rows), _ACT[dtype], k.data_ptr(), v.data_ptr(),
-                                  self.kv_heads * self.head_dim, self.head_dim, self._stream()))
+        n, heads, hd = len(seqs), self.kv_heads, self.head_dim
+        rows = _lib.KvRowsC(n, self._index(seqs, n, "seqs"), self._index(positions, n, "positions"))
+        k = torch.empty((n, heads, hd), dtype=dtype, device=self.pages.device)
+        v = torch.empty_like(k)
+        status = lib().chonk_kv_read(self._c, C.byref(rows), _ACT[dtype], k.data_ptr(), v.data_ptr(), heads * hd, hd,
+                                     _stream(self._at))
+        if status:
+            check(status)
         return k, v
 
     def attend(self, q: torch.Tensor, seqs: torch.Tensor, lengths: torch.Tensor, *, scale: Optional[float] = None,
@@ -167,23 +186,27 @@ class PagedKv:
         """Attention of rows q [n, heads, head_dim] over the first lengths[i] positions of
         sequence seqs[i] (the last `window` of them where given). Length 0 gives zeros; rows
         with a negative sequence are left out."""
-        n, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
-        q_ld = self._rows(q, None, None, "q")
+        if q.dim() != 3 or q.dtype not in _ACT:
+            _refuse("q must be float32 or float16 [n, heads, head_dim]")
+        dtype, (n, heads, hd) = q.dtype, q.shape
+        q_ld = self._rows(q, n, heads, dtype, "q")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
-        o_ld = self._rows(out, heads, q.dtype, "out")
-        if out.shape[0] != n:
-            _refuse("q and out differ in rows")
-        seqs, lengths = self._index(seqs, n, "seqs"), self._index(lengths, n, "lengths")
+            out, o_ld = torch.empty_like(q, memory_format=torch.contiguous_format), heads * hd
+        else:
+            o_ld = self._rows(out, n, heads, dtype, "out")
         L = lib()
-        need = L.chonk_kv_attend_workspace(C.byref(self._c), n, heads)
-        if need < 0:
+        need, work, work_at = L.chonk_kv_attend_workspace(self._c, n, heads), None, None
+        if need > 0:
+            work = torch.empty(need, dtype=torch.uint8, device=self.pages.device)
+            work_at = work.data_ptr()
+        elif need < 0:
             check(need)
-        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        a = _lib.KvAttendArgsC(_ACT[q.dtype], heads, n, seqs.data_ptr(), lengths.data_ptr(), q.data_ptr(),
-                               out.data_ptr(), q_ld, o_ld, self.head_dim ** -0.5 if scale is None else scale, window,
-                               work.data_ptr() if work is not None else None, need)
-        check(L.chonk_kv_attend(C.byref(self._c), C.byref(a), self._stream()))
+        a = _lib.KvAttendArgsC(_ACT[dtype], heads, n, self._index(seqs, n, "seqs"), self._index(lengths, n, "lengths"),
+                               q.data_ptr(), out.data_ptr(), q_ld, o_ld, hd ** -0.5 if scale is None else scale, window,
+                               work_at, need)
+        status = L.chonk_kv_attend(self._c, C.byref(a), _stream(self._at))
+        if status:
+            check(status)
         return out
 
     def check(self) -> None:
