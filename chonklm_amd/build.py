@@ -2,7 +2,8 @@
 
 Run ``python -m chonklm_amd.build`` or call :func:`build_all`. Outputs stay
 in-tree (``chonklm_amd/_lib/libchonk.so``, the Node addon
-``chonklm_amd/_lib/chonk_napi.node``, ``oracle/_build/liborc.so``) so that
+``chonklm_amd/_lib/chonk_napi.node``, the paged K/V cache's Python calls
+``chonklm_amd/_lib/_paged_kv.so``, ``oracle/_build/liborc.so``) so that
 they travel with the repository snapshot to the GPU host.
 """
 from __future__ import annotations
@@ -12,6 +13,7 @@ import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -121,6 +123,27 @@ def build_napi() -> Path | None:
     return NAPI_PATH
 
 
+PAGED_KV_SOURCE = PKG / "csrc/torch_kv/paged_kv_ext.cpp"
+PAGED_KV_PATH = LIB_DIR / "_paged_kv.so"
+
+
+def build_paged_kv() -> Path | None:
+    """Builds the Python calls of the paged K/V cache over libchonk.so (skipped where torch is absent)."""
+    try:
+        import torch
+    except ImportError:
+        return None
+    base = Path(torch.__file__).resolve().parent
+    tmp = PAGED_KV_PATH.with_suffix(".so.tmp")
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{ROOT / 'include'}",
+          "-isystem", str(base / "include"), "-isystem", sysconfig.get_paths()["include"], str(PAGED_KV_SOURCE),
+          "-o", str(tmp), f"-L{LIB_DIR}", "-lchonk", f"-L{base / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10",
+          "-Wl,-rpath,$ORIGIN"])
+    os.replace(tmp, PAGED_KV_PATH)
+    return PAGED_KV_PATH
+
+
 def build_oracle() -> Path | None:
     """Builds the oracle's CPU restatement (test infrastructure)."""
     oracle = ROOT / "oracle"
@@ -133,6 +156,7 @@ def build_oracle() -> Path | None:
 def build_all(jobs: int = 8) -> None:
     build_library(jobs)
     build_napi()
+    build_paged_kv()
     build_oracle()
 
 
