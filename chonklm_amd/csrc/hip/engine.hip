@@ -40,6 +40,7 @@
 #include "chonk.h"
 #include "errors.h"
 #include "kernels.h"
+#include "paged_kv.h"
 #include "prefill.h"
 
 // Row buffers of the no-allocation prompt pass (chonk_engine_prefill_noalloc):
@@ -2372,6 +2373,12 @@ struct RowKv {
   int ctx = 0;
   const int32_t* pages = nullptr;
   int max_pages = 0;
+  // 8- or 4-bit pages (paged_kv.h) instead: kc[i] is layer i's pool, vc is empty, and a
+  // prompt's attention reads the sequence's values from back_k / back_v, one layer's
+  // [kv_heads][ctx][hd] in fp16
+  int coded = 0;  // CHONK_KV_Q8 or CHONK_KV_Q4, 0: fp16 pages
+  int n_pages = 0, n_seqs = 0;
+  void *back_k = nullptr, *back_v = nullptr;
 };
 
 // Where the rows sit: positions p0 + row of sequence seq0, or per-row arrays.
@@ -2380,6 +2387,9 @@ struct RowPlace {
   const int32_t* row_seq = nullptr;  // device [rows]
   const int32_t* row_pos = nullptr;  // device [rows]
 };
+
+// The first position that a row at `pos` sees through a window (0: none).
+int at_window(int window, int pos) { return window > 0 ? std::max(0, pos + 1 - window) : 0; }
 
 // The layers for rows 0..T-1 whose token ids are in b.tok: every layer's K/V
 // of the rows into the cache; with logits != null also the last layer's
@@ -2469,7 +2479,7 @@ void run_rows(chonk_engine* e, const RowBufs& b, const RowKv& kvs, const RowPlac
   auto kv_addr = [&](int i) {
     KvAddr k{};
     k.kc = kvs.kc[i];
-    k.vc = kvs.vc[i];
+    k.vc = kvs.coded ? nullptr : kvs.vc[i];
     k.ctx = kvs.ctx;
     k.pages = kvs.pages;
     k.max_pages = kvs.max_pages;
@@ -2584,38 +2594,122 @@ void run_rows(chonk_engine* e, const RowBufs& b, const RowKv& kvs, const RowPlac
       // (the decode attention's table, made with the engine)
       r.rope_cs = e->dec_attn ? rope_cs_table(e, c.layer[i].theta, c.hd) : nullptr;
       r.kv = kv_addr(i);
-      // decode batches: the page-walking attention (one workgroup per (kv head,
-      // row) walking all of its pages also does the rotary/K-V write)
-      const bool walk = pl.row_seq && c.hd >= 64 && lc.heads / lc.kv_heads <= 8 && kvs.max_pages <= 64;
-      const bool fuse_rope = walk && !last_kv && bd_attn_segments(T, lc.kv_heads, kvs.max_pages) == 1;
-      if (!fuse_rope) HIP_OK(launch_pf_rope_kv(r, T, s));
-      if (last_kv) break;
-      PfAttnArgs at{};
-      at.qkv = b.qkv;
-      at.ld = ldqkv;
-      at.out = b.att;
-      at.ldo = qdim;
-      at.heads = lc.heads;
-      at.kv_heads = lc.kv_heads;
-      at.hd = c.hd;
-      at.window = c.layer[i].window;
-      at.kv16 = r.kv16;
-      at.scale = c.scale;
-      at.kv = r.kv;
-      bool planes = false;  // the attention wrote the o-projection's operand planes
-      if (walk) {
-        // (the walk writes no sums of x)
-        if (!gemm_needs_sums(L.o.q.type, qdim, T)) {
-          at.oh = b.h;
-          at.ol = b.l;
-          at.oscale = b.xscale;
-          at.okpad = gemm_kpad(qdim);
+      if (kvs.coded) {
+        KvAppendArgs w{};
+        w.c.pages = (uint8_t*)kvs.kc[i];
+        w.c.table = kvs.pages;
+        w.c.type = kvs.coded;
+        w.c.kv_heads = lc.kv_heads;
+        w.c.hd = c.hd;
+        w.c.n_pages = kvs.n_pages;
+        w.c.n_seqs = kvs.n_seqs;
+        w.c.max_pages = kvs.max_pages;
+        w.at.seq = pl.row_seq;
+        w.at.pos = pl.row_pos;
+        w.at.seq0 = pl.seq0;
+        w.at.p0 = pl.p0;
+        w.q = r.pq;
+        w.k = r.pk;
+        w.v = r.pv;
+        w.q_ld = r.pq.ld;
+        w.k_ld = r.pk.ld;
+        w.v_ld = r.pv.ld;
+        w.q_out = b.qkv;
+        w.qo_ld = ldqkv;
+        w.rows = T;
+        w.heads = lc.heads;
+        w.qn_w = r.qn_w;
+        w.kn_w = r.kn_w;
+        w.eps = c.qk_eps;
+        w.rope = rope_cs_table(e, c.layer[i].theta, c.hd);
+        w.rope_dim = c.hd;
+        w.rope_n = c.ctx;
+        w.interleaved = r.interleaved;
+        HIP_OK(launch_kv_append(w, s));
+        if (last_kv) break;
+        if (pl.row_seq) {
+          KvAttendArgs at{};
+          at.c = w.c;
+          at.seq = pl.row_seq;
+          at.len = pl.row_pos;
+          at.len_add = 1;
+          at.q = b.qkv;
+          at.q_ld = ldqkv;
+          at.out = b.att;
+          at.o_ld = qdim;
+          at.rows = T;
+          at.heads = lc.heads;
+          at.window = c.layer[i].window;
+          at.scale = c.scale;
+          at.part = b.part;
+          if (kv_attend_floats(at.c, T, lc.heads) > P) throw Error(CHONK_EINVAL, "partial sums do not fit the row buffers");
+          HIP_OK(launch_kv_attend(at, s));
+        } else {
+          // from the key block (64 positions) of the first one that row 0 sees
+          const int lo = at_window(c.layer[i].window, pl.p0) / kKvPage * kKvPage;
+          KvReadArgs rd{};
+          rd.c = w.c;
+          rd.at.seq0 = pl.seq0;
+          rd.at.p0 = lo;
+          rd.rows = pl.p0 + T - lo;
+          rd.k = (uint16_t*)kvs.back_k + (size_t)lo * c.hd;
+          rd.v = (uint16_t*)kvs.back_v + (size_t)lo * c.hd;
+          rd.row_ld = c.hd;
+          rd.head_ld = (int64_t)kvs.ctx * c.hd;
+          rd.f16 = 1;
+          HIP_OK(launch_kv_read(rd, s));
+          PfAttnArgs at{};
+          at.qkv = b.qkv;
+          at.ld = ldqkv;
+          at.out = b.att;
+          at.ldo = qdim;
+          at.heads = lc.heads;
+          at.kv_heads = lc.kv_heads;
+          at.hd = c.hd;
+          at.window = c.layer[i].window;
+          at.kv16 = 1;
+          at.scale = c.scale;
+          at.kv.kc = kvs.back_k;
+          at.kv.vc = kvs.back_v;
+          at.kv.ctx = kvs.ctx;
+          at.kv.p0 = pl.p0;
+          HIP_OK(launch_pf_attn(at, T, s));
         }
-        HIP_OK(launch_bd_attn(at, T, b.part, P, s, &planes, fuse_rope ? &r : nullptr));
+        split(b.att, qdim, qdim, nullptr, T, PartSum{}, nullptr);
       } else {
-        HIP_OK(launch_pf_attn(at, T, s));
+        // decode batches: the page-walking attention (one workgroup per (kv head,
+        // row) walking all of its pages also does the rotary/K-V write)
+        const bool walk = pl.row_seq && c.hd >= 64 && lc.heads / lc.kv_heads <= 8 && kvs.max_pages <= 64;
+        const bool fuse_rope = walk && !last_kv && bd_attn_segments(T, lc.kv_heads, kvs.max_pages) == 1;
+        if (!fuse_rope) HIP_OK(launch_pf_rope_kv(r, T, s));
+        if (last_kv) break;
+        PfAttnArgs at{};
+        at.qkv = b.qkv;
+        at.ld = ldqkv;
+        at.out = b.att;
+        at.ldo = qdim;
+        at.heads = lc.heads;
+        at.kv_heads = lc.kv_heads;
+        at.hd = c.hd;
+        at.window = c.layer[i].window;
+        at.kv16 = r.kv16;
+        at.scale = c.scale;
+        at.kv = r.kv;
+        bool planes = false;  // the attention wrote the o-projection's operand planes
+        if (walk) {
+          // (the walk writes no sums of x)
+          if (!gemm_needs_sums(L.o.q.type, qdim, T)) {
+            at.oh = b.h;
+            at.ol = b.l;
+            at.oscale = b.xscale;
+            at.okpad = gemm_kpad(qdim);
+          }
+          HIP_OK(launch_bd_attn(at, T, b.part, P, s, &planes, fuse_rope ? &r : nullptr));
+        } else {
+          HIP_OK(launch_pf_attn(at, T, s));
+        }
+        if (!planes) split(b.att, qdim, qdim, nullptr, T, PartSum{}, nullptr);
       }
-      if (!planes) split(b.att, qdim, qdim, nullptr, T, PartSum{}, nullptr);
       po = gemm(L.o, T, 0, P);
     }
     // x += o (Gemma-3: x = clamp(x + RMSNorm(o) * post_norm)), then the ffn norm
@@ -3735,7 +3829,7 @@ int chonk_write_shards(const char* gguf_path, const char* out_dir, uint64_t shar
 struct chonk_batch {
   chonk_engine* e = nullptr;
   int max_seqs = 0, max_tokens = 0, max_pages = 0, rows_cap = 0;
-  void* kv_mem = nullptr;   // per layer: K pages | V pages, [page][kv_heads][64][hd] fp16
+  void* kv_mem = nullptr;   // per layer: K pages | V pages, [page][kv_heads][64][hd] fp16, or coded pages
   void* row_mem = nullptr;  // row buffers, page table, row arrays, logits
   int32_t *pages = nullptr, *rseq = nullptr, *rpos = nullptr, *next = nullptr;
   float* logits = nullptr;  // [max(max_seqs, 1)][vocab], rows of the last call
@@ -3759,7 +3853,7 @@ void batch_free(chonk_batch* b) {
   delete b;
 }
 
-void batch_create(chonk_engine* e, int max_seqs, int max_tokens, chonk_batch** out) {
+void batch_create(chonk_engine* e, int max_seqs, int max_tokens, int kv_type, chonk_batch** out) {
   const ModelCfg& c = e->cfg;
   if (max_seqs <= 0 || max_seqs > 1024 || max_tokens <= 0 || max_tokens > c.ctx)
     throw Error(CHONK_EINVAL, "batch needs 1..1024 sequences of 1.." + std::to_string(c.ctx) + " tokens");
@@ -3771,6 +3865,11 @@ void batch_create(chonk_engine* e, int max_seqs, int max_tokens, chonk_batch** o
   if (e->kv_elem != 2) throw Error(CHONK_EINVAL, "batched decoding needs the fp16 K/V cache");
   if (c.heads / c.kv_heads > 16) throw Error(CHONK_EINVAL, "batched decoding supports GQA groups up to 16");
   if (c.openelm) throw Error(CHONK_EINVAL, "batched decoding needs one head geometry for every layer (not openelm)");
+  if (!kv_type_ok(kv_type))
+    throw Error(CHONK_EINVAL, "batched decoding needs an fp16, 8-bit or 4-bit K/V cache, not kv type " + std::to_string(kv_type));
+  const bool coded = kv_type != CHONK_KV_F16;
+  if (coded && !kv_hd_ok(c.hd))
+    throw Error(CHONK_EINVAL, "8- and 4-bit K/V caches need head_dim 32, 64, 128 or 256, not " + std::to_string(c.hd));
   std::unique_ptr<chonk_batch, void (*)(chonk_batch*)> b(new chonk_batch(), batch_free);
   b->e = e;
   b->max_seqs = max_seqs;
@@ -3779,14 +3878,30 @@ void batch_create(chonk_engine* e, int max_seqs, int max_tokens, chonk_batch** o
   b->rows_cap = std::max(kPrefillRows, max_seqs);
   b->len.assign((size_t)max_seqs, 0);
   const size_t n_pages = (size_t)max_seqs * b->max_pages;
-  const size_t pool = align256(n_pages * c.kv_heads * kKvPage * c.hd * 2);
-  HIP_OK(hipMalloc(&b->kv_mem, pool * 2 * c.layers));
-  HIP_OK(hipMemset(b->kv_mem, 0, pool * 2 * c.layers));  // finite values in slots not yet written
   b->kvs.ctx = max_tokens;
   b->kvs.max_pages = b->max_pages;
-  for (int i = 0; i < c.layers; ++i) {
-    b->kvs.kc.push_back((uint8_t*)b->kv_mem + pool * 2 * i);
-    b->kvs.vc.push_back((uint8_t*)b->kv_mem + pool * (2 * i + 1));
+  if (coded) {
+    const size_t pool = align256(n_pages * c.kv_heads * 2 * kv_part_bytes(kv_type, c.hd));
+    const size_t back = align256((size_t)c.kv_heads * max_tokens * c.hd * 2);
+    HIP_OK(hipMalloc(&b->kv_mem, pool * c.layers + 2 * back));
+    HIP_OK(hipMemset(b->kv_mem, 0, pool * c.layers + 2 * back));
+    b->kvs.coded = kv_type;
+    b->kvs.n_pages = (int)n_pages;
+    b->kvs.n_seqs = max_seqs;
+    for (int i = 0; i < c.layers; ++i) {
+      b->kvs.kc.push_back((uint8_t*)b->kv_mem + pool * i);
+      (void)rope_cs_table(e, c.layer[i].theta, c.hd);  // (made here: a step under capture cannot allocate it)
+    }
+    b->kvs.back_k = (uint8_t*)b->kv_mem + pool * c.layers;
+    b->kvs.back_v = (uint8_t*)b->kvs.back_k + back;
+  } else {
+    const size_t pool = align256(n_pages * c.kv_heads * kKvPage * c.hd * 2);
+    HIP_OK(hipMalloc(&b->kv_mem, pool * 2 * c.layers));
+    HIP_OK(hipMemset(b->kv_mem, 0, pool * 2 * c.layers));  // finite values in slots not yet written
+    for (int i = 0; i < c.layers; ++i) {
+      b->kvs.kc.push_back((uint8_t*)b->kv_mem + pool * 2 * i);
+      b->kvs.vc.push_back((uint8_t*)b->kv_mem + pool * (2 * i + 1));
+    }
   }
   const int64_t part = row_part_floats(c, b->rows_cap);
   const size_t rb = row_bufs_layout(c, b->rows_cap, part, nullptr, nullptr);
@@ -3897,9 +4012,13 @@ void batch_step(chonk_batch* b, const int32_t* seqs, const int32_t* tokens, size
 }  // namespace chonk
 
 int chonk_batch_create(chonk_engine* e, int32_t max_seqs, int32_t max_tokens, chonk_batch** out) {
+  return chonk_batch_create_kv(e, max_seqs, max_tokens, CHONK_KV_F16, out);
+}
+
+int chonk_batch_create_kv(chonk_engine* e, int32_t max_seqs, int32_t max_tokens, int32_t kv_type, chonk_batch** out) {
   if (!out) return CHONK_EINVAL;
   *out = nullptr;
-  return api(e, [&] { batch_create(e, max_seqs, max_tokens, out); });
+  return api(e, [&] { batch_create(e, max_seqs, max_tokens, kv_type, out); });
 }
 
 int chonk_batch_destroy(chonk_batch* b) {

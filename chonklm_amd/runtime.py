@@ -203,14 +203,21 @@ def load_llama_wgsl_model(model: ModelDef, on_progress: Optional[Callable] = Non
 class LlamaWgslBatch:
     """Independent sequences decoded together over one engine's weights (no
     counterpart in the reference, which runs one sequence per engine): each
-    sequence has its own paged fp16 K/V cache; a step appends one token to any
+    sequence has its own paged K/V cache, in fp16 ("f16") or 8- or 4-bit codes ("q8",
+    "q4": about a half or 0.28 of the bytes); a step appends one token to any
     subset of them and returns their greedy next ids (chonk_batch_*)."""
 
-    def __init__(self, engine: LlamaWgslEngine, max_seqs: int, max_tokens: int):
+    KV_TYPES = {"f16": _lib.KV_F16, "q8": _lib.KV_Q8, "q4": _lib.KV_Q4}
+
+    def __init__(self, engine: LlamaWgslEngine, max_seqs: int, max_tokens: int, kv_dtype: str = "f16"):
+        if kv_dtype not in self.KV_TYPES:
+            raise ChonkError(_lib.CHONK_EINVAL, f"batched decoding: unsupported kv_dtype {kv_dtype!r}")
+        self._h = None
         self.engine = engine
         self.vocab = engine.info["vocab"]
         h = C.c_void_p()
-        check(lib().chonk_batch_create(engine._h, int(max_seqs), int(max_tokens), C.byref(h)), engine._h)
+        check(lib().chonk_batch_create_kv(engine._h, int(max_seqs), int(max_tokens), self.KV_TYPES[kv_dtype], C.byref(h)),
+              engine._h)
         self._h = h
 
     def prefill(self, seq: int, token_ids: Sequence[int]) -> int:

@@ -238,12 +238,18 @@ int chonk_engine_fake_context(chonk_engine* e, int32_t pos, uint64_t seed);
 /* Batched decoding (no counterpart in the reference, which runs one sequence
  * per engine) -----------------------------------------------------------------
  * Independent sequences over one engine's weights, each with its own paged
- * fp16 K/V cache (pages of 64 positions); one step advances any subset of the
+ * K/V cache (pages of 64 positions, fp16 unless chonk_batch_create_kv says otherwise); one step advances any subset of the
  * sequences by one token, every linear layer a dequant-fused MFMA GEMM over
  * the batch rows. Greedy selection (argmax, no repetition penalty). The
  * engine's own conversation is not touched. */
 typedef struct chonk_batch chonk_batch;
 int chonk_batch_create(chonk_engine* e, int32_t max_seqs, int32_t max_tokens_per_seq, chonk_batch** out);
+/* The same with the pages of kv_type CHONK_KV_F16, CHONK_KV_Q8 or CHONK_KV_Q4 (the paged
+ * caches below; head_dim 32, 64, 128 or 256): 8 or 4 bits hold 1.9 or 3.6
+ * times the positions in the same memory. Steps attend over the codes' values, a
+ * prompt's rows over them rounded to fp16. */
+int chonk_batch_create_kv(chonk_engine* e, int32_t max_seqs, int32_t max_tokens_per_seq, int32_t kv_type,
+                          chonk_batch** out);
 int chonk_batch_destroy(chonk_batch* b);
 /* Starts sequence `seq` over: K/V of the prompt, and the greedy next id. */
 int chonk_batch_prefill(chonk_batch* b, int32_t seq, const int32_t* tokens, size_t n, int32_t* next_id);
