@@ -32,7 +32,8 @@ typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kMostWgs = 1024;  // segments of a split attention, at most
-constexpr int kMinHalves = 16;  // ... of at least so many half pages
+constexpr int kWholeHalves = 32;  // half pages of a row that is never cut
+constexpr int kMinHalves = 8;   // ... of at least so many half pages
 
 __device__ __forceinline__ f4_t mfma(h8_t a, h8_t b, f4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -588,7 +589,7 @@ struct Span {
 };
 
 // The rows' cut into segments, the same in every wave: at most `want`
-// segments of about as many halves each, found from all the rows' lengths, so that
+// segments (at least kMinHalves long) of about as many halves each, found from all the rows' lengths, so that
 // ragged rows keep the device as evenly busy as equal ones and the host needs to know no
 // length. A lane looks at rows 4 lane .. 4 lane + 3 (at most 256 rows). The row that
 // `mine` holds for comes back in all lanes (row -1: none).
@@ -611,17 +612,33 @@ __device__ __forceinline__ Cut cut_rows(const KvAttendArgs& a, int items, F mine
     const Span s(a, seq[i], len[i], false);
     n[i] = r0 + i < a.rows ? s.h1 - s.h0 : 0;
   }
-  // (as floats: a bound that is a little off only makes segments a little longer)
+  // The shortest length of a segment that leaves at most `want` of them: between an
+  // even share and what must do (every item's last segment may be short), by halving. As
+  // floats: whatever the length, the segments it gives are the same in every wave.
   float total = 0.f;
 #pragma unroll
   for (int i = 0; i < R; ++i) total += (float)n[i];
   total = wave_sum(total) * (float)items;
-  const int room = a.want - a.rows * items;
-  const int most = max(kMinHalves, (int)fminf(total / (float)room * 1.0001f + 1.f, 1e9f));
+  const float want = (float)a.want;
+  float lo = total / want, hi = total / (want - (float)(a.rows * items)) * 1.0001f + 1.f;
+  auto pieces = [&](int i, float most) { return r0 + i < a.rows ? max(1, (int)ceilf((float)n[i] / most)) : 0; };
+  if (hi > (float)kMinHalves) {
+    for (int k = 0; k < 4; ++k) {
+      const float mid = 0.5f * (lo + hi);
+      int t = 0;
+#pragma unroll
+      for (int i = 0; i < R; ++i) t += pieces(i, mid);
+      if (wave_sum((float)t) * (float)items <= want)
+        hi = mid;
+      else
+        lo = mid;
+    }
+  }
+  const float most = fmaxf(hi, (float)kMinHalves);
   int segs[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    segs[i] = r0 + i < a.rows ? max(1, (int)((uint32_t)(n[i] + most - 1) / (uint32_t)most)) : 0;
+    segs[i] = pieces(i, most);
     sum += segs[i];
   }
   int before = sum;
@@ -670,29 +687,32 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 }
 
 // One workgroup per segment of a (row, kv head, up to 16 of its q heads); its
-// four waves take the segment's half pages in turn, each with its own running
+// NW waves take the segment's half pages in turn, each with its own running
 // maximum, sum and output, and meet in LDS at the end.
 //
-// PACK (at most four heads): the products have 16 columns for them, and what is done to
-// the scores between the products (exponentials, weights times V's scales,
-// their split into two halves) would be done on all 16. So the scores of a half
-// page, 4 heads x 32 positions, go through LDS to two a lane, and the split
-// weights back; the idle columns get a copy of the others.
-template <int KV, int NB, bool PACK>
-__global__ __launch_bounds__(kWg, NB == 8 ? 2 : NB == 4 ? 3 : 4) void k_kv_attend(KvAttendArgs a) {
-  constexpr int HD = 32 * NB, PART = kv_part_bytes(KV, HD);
+// q and the weights are split into two fp16 halves each, hi + lo. With more than four heads
+// that is two products. PACK (at most four heads): the products have 16 columns for
+// them, so columns 0 .. 3 take the heads' hi and 4 .. 7 their lo in one product (8 .. 15 a copy);
+// and as what is done to the scores between the products (exponentials, weights times
+// V's scales, their split) would be done on all 16, the scores of a half page, 4 heads
+// x 32 positions, go through LDS to two a lane, and the split weights back. Half the
+// products and a third fewer vector instructions.
+template <int KV, int NB, bool PACK, int NW>
+__global__ __launch_bounds__(64 * NW, NB == 8 ? 2 : NB == 4 ? (NW == 8 ? 2 : 3) : 4) void k_kv_attend(KvAttendArgs a) {
+  constexpr int HD = 32 * NB, PART = kv_part_bytes(KV, HD), WG = 64 * NW;
   constexpr bool F = KV == CHONK_KV_F16;
   constexpr int WB = F ? 1 : NB;            // blocks with weights of their own
   // What registers cannot hold beside K and V of a half page and the output: q's halves
   // go to LDS, and fp16's 256-wide rows are fetched one of K and V at a time.
-  constexpr bool QL = NB == 8 || (NB == 4 && KV != CHONK_KV_Q4);
+  constexpr bool QL = NB == 8 || (NB == 4 && KV != CHONK_KV_Q4 && !PACK);
+  constexpr int QP = PACK ? 1 : 2;          // halves of q that a lane holds
   constexpr bool ONE = F && NB == 8;
   extern __shared__ __align__(16) float sm[];  // [wave][head][HD] | [wave][head][m, l]
-  __shared__ __align__(16) uint32_t sck[4][F ? 4 : NB * 16];          // K's scales, as stored
-  __shared__ __align__(16) uint32_t scv[4][F ? 4 : NB * 16];          // V's (PACK: [pair][block])
-  __shared__ __align__(16) float ss[4][PACK ? 4 * 32 : 4];            // scores [head][place]
-  __shared__ __align__(16) uint32_t sw[4][PACK ? WB * 2 * 64 : 4];    // weights [block][hi, lo][head][16 pairs]
-  __shared__ __align__(16) uint32_t sq[QL ? NB * 2 * 64 * 4 : 4];
+  __shared__ __align__(16) uint32_t sck[NW][F ? 4 : NB * 16];          // K's scales, as stored
+  __shared__ __align__(16) uint32_t scv[NW][F ? 4 : NB * 16];          // V's (PACK: [pair][block])
+  __shared__ __align__(16) float ss[NW][PACK ? 8 * 32 : 4];            // scores [column][place]
+  __shared__ __align__(16) uint32_t sw[NW][PACK ? WB * 2 * 64 : 4];    // weights [block][hi, lo][head][16 pairs]
+  __shared__ __align__(16) uint32_t sq[QL ? NB * QP * 64 * 4 : 4];
   const int G = a.heads / a.c.kv_heads, hgs = (G + 15) / 16, items = a.c.kv_heads * hgs;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, col = lane & 15;
@@ -741,11 +761,11 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 2 : NB == 4 ? 3 : 4) void k_kv_atten
 
   // q: this lane's head at dims 32 b + 8 g + e, scaled by a power of two so that the
   // head's largest lies in [2^13, 2^14) and split into two halves of 11 bits each
-  h8_t qh[QL ? 1 : NB], ql[QL ? 1 : NB];
+  h8_t qr[QL ? 1 : NB][QP];
   float mul;             // score of S in powers of two
   {
     float x[NB][8];
-    const int h = h0 + min(col, nh - 1);
+    const int h = h0 + min(PACK ? col & 3 : col, nh - 1);
     const int64_t o = r * a.q_ld + (int64_t)h * HD + 8 * g;
     float top = 0.f;
 #pragma unroll
@@ -775,14 +795,15 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 2 : NB == 4 ? 3 : 4) void k_kv_atten
         hi[e] = (_Float16)y;
         lo[e] = (_Float16)(y - (float)hi[e]);
       }
+      if constexpr (PACK) hi = col & 4 ? lo : hi;
       if constexpr (QL) {
         if (wave == 0) {
-          *(h8_t*)(sq + (2 * b * 64 + lane) * 4) = hi;
-          *(h8_t*)(sq + ((2 * b + 1) * 64 + lane) * 4) = lo;
+          *(h8_t*)(sq + (QP * b * 64 + lane) * 4) = hi;
+          if constexpr (!PACK) *(h8_t*)(sq + ((QP * b + 1) * 64 + lane) * 4) = lo;
         }
       } else {
-        qh[b] = hi;
-        ql[b] = lo;
+        qr[b][0] = hi;
+        if constexpr (!PACK) qr[b][1] = lo;
       }
     }
   }
@@ -803,10 +824,10 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 2 : NB == 4 ? 3 : 4) void k_kv_atten
 #pragma unroll
   for (int i = 0; i < 2 * NB; ++i) acc[i] = f4_t{0.f, 0.f, 0.f, 0.f};
 
-  for (; hx < to; hx += 4) {
+  for (; hx < to; hx += NW) {
     const int j0 = 32 * hx;
     const bool edge = j0 < sp.first || j0 + 32 > sp.len;
-    const bool more = hx + 4 < to;
+    const bool more = hx + NW < to;
     if constexpr (!F) {
       constexpr int D = NB == 8 ? 2 : 1;
       if (edge) {  // scales of unseen places may be anything
@@ -847,18 +868,19 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 2 : NB == 4 ? 3 : 4) void k_kv_atten
     for (int e = 0; e < 8; ++e) s[e] = 0.f;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      h8_t k0, k1, hi, lo;
+      h8_t k0, k1;
       kc.k_tiles(b, k0, k1);
-      if constexpr (QL) {
-        hi = *(const h8_t*)(sq + (2 * b * 64 + lane) * 4);
-        lo = *(const h8_t*)(sq + ((2 * b + 1) * 64 + lane) * 4);
-      } else {
-        hi = qh[b];
-        lo = ql[b];
+      f4_t s0 = f4_t{0.f, 0.f, 0.f, 0.f}, s1 = s0;
+#pragma unroll
+      for (int i = 0; i < QP; ++i) {
+        h8_t q;
+        if constexpr (QL)
+          q = *(const h8_t*)(sq + ((QP * b + i) * 64 + lane) * 4);
+        else
+          q = qr[b][i];
+        s0 = mfma(k0, q, s0);
+        s1 = mfma(k1, q, s1);
       }
-      const f4_t z = f4_t{0.f, 0.f, 0.f, 0.f};
-      const f4_t s0 = mfma(k0, lo, mfma(k0, hi, z));
-      const f4_t s1 = mfma(k1, lo, mfma(k1, hi, z));
       if constexpr (F) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -874,8 +896,8 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 2 : NB == 4 ? 3 : 4) void k_kv_atten
         }
       }
     }
-    // (4 halves on: the same half of its page)
-    const uint8_t* next = ONE ? part_of(hx) : more ? part_of(hx + 4) : nullptr;
+    // (an even number of halves on: the same half of its page)
+    const uint8_t* next = ONE ? part_of(hx) : more ? part_of(hx + NW) : nullptr;
     if constexpr (ONE)
       vc.load(next + PART, hx & 1, lane);
     else if (more)
@@ -911,14 +933,14 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 2 : NB == 4 ? 3 : 4) void k_kv_atten
     }
     float s0 = 0.f, s1 = 0.f, top;
     if constexpr (PACK) {
-      if (col < 4) {
+      if (col < 8) {
         *(float4*)(ss[wave] + col * 32 + 8 * g) = make_float4(s[0], s[1], s[2], s[3]);
         *(float4*)(ss[wave] + col * 32 + 8 * g + 4) = make_float4(s[4], s[5], s[6], s[7]);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      s0 = ss[wave][hc * 32 + pa];
-      s1 = ss[wave][hc * 32 + pb];
+      s0 = ss[wave][hc * 32 + pa] + ss[wave][(hc + 4) * 32 + pa];
+      s1 = ss[wave][hc * 32 + pb] + ss[wave][(hc + 4) * 32 + pb];
       top = group_max<16>(fmaxf(s0, s1));
     } else {
       top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
@@ -967,18 +989,17 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 2 : NB == 4 ? 3 : 4) void k_kv_atten
         l += p[e];
       }
     }
-    uint32_t ph[4], pl[4];
+    [[maybe_unused]] uint32_t ph[4], pl[4];
     if constexpr (F && !PACK) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) split2(p[2 * i], p[2 * i + 1], ph[i], pl[i]);
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      h8_t wh, wl, v0, v1;
+      h8_t wh, v0, v1;
+      vc.v_tiles(b, v0, v1);
       if constexpr (PACK) {
-        const uint32_t* x = sw[wave] + 2 * (F ? 0 : b) * 64 + (col & 3) * 16 + 4 * g;
-        wh = *(const h8_t*)x;
-        wl = *(const h8_t*)(x + 64);
+        wh = *(const h8_t*)(sw[wave] + (2 * (F ? 0 : b) + (col >> 2 & 1)) * 64 + (col & 3) * 16 + 4 * g);
       } else {
         if constexpr (!F) {
           const uint4 d = *(const uint4*)(scv[wave] + b * 16 + g * 4);
@@ -988,20 +1009,26 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 2 : NB == 4 ? 3 : 4) void k_kv_atten
           split2(mul_half<1>(p[5], d.z), mul_half<1>(p[7], d.w), ph[3], pl[3]);
         }
         wh = halves(ph[0], ph[1], ph[2], ph[3]);
-        wl = halves(pl[0], pl[1], pl[2], pl[3]);
+        const h8_t wl = halves(pl[0], pl[1], pl[2], pl[3]);
+        acc[2 * b] = mfma(v0, wl, acc[2 * b]);
+        acc[2 * b + 1] = mfma(v1, wl, acc[2 * b + 1]);
       }
-      vc.v_tiles(b, v0, v1);
-      acc[2 * b] = mfma(v0, wl, mfma(v0, wh, acc[2 * b]));
-      acc[2 * b + 1] = mfma(v1, wl, mfma(v1, wh, acc[2 * b + 1]));
+      acc[2 * b] = mfma(v0, wh, acc[2 * b]);
+      acc[2 * b + 1] = mfma(v1, wh, acc[2 * b + 1]);
     }
     if constexpr (ONE) {
-      if (more) kc.load(part_of(hx + 4), hx & 1, lane);
+      if (more) kc.load(part_of(hx + NW), hx & 1, lane);
     } else if (more) {
       vc.load(next + PART, hx & 1, lane);
     }
   }
   if constexpr (PACK) {
     l = group_sum<16>(l);
+    // column c + 4 into column c: the lo weights' share
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][e] += dpp<0x104>(acc[i][e]);
   } else {
     float t0, t1;
     swap16(l, t0, t1);
@@ -1011,7 +1038,7 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 2 : NB == 4 ? 3 : 4) void k_kv_atten
   }
   if (poison) l = __builtin_nanf("");
   // the waves' rows meet in LDS
-  float* ml = sm + 4 * nh * HD;
+  float* ml = sm + NW * nh * HD;
   if (col < nh) {
     float* o = sm + (wave * nh + col) * HD;
 #pragma unroll
@@ -1030,14 +1057,14 @@ __global__ __launch_bounds__(kWg, NB == 8 ? 2 : NB == 4 ? 3 : 4) void k_kv_atten
   const int nhm = min(G, 16);
   float* prow = a.part + (int64_t)blockIdx.x * nhm * HD;
   float* pml = a.part + (int64_t)a.want * nhm * HD + (int64_t)blockIdx.x * nhm * 2;
-  for (int x = tid; x < nh * HD; x += kWg) {
+  for (int x = tid; x < nh * HD; x += WG) {
     const int h = x / HD, d = x % HD;
     float M = -1e30f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, ml[(w * nh + h) * 2]);
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[(w * nh + h) * 2]);
     float L = 0.f, O = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float f = __builtin_amdgcn_exp2f(ml[(w * nh + h) * 2] - M);
       L += f * ml[(w * nh + h) * 2 + 1];
       O += f * sm[(w * nh + h) * HD + d];
@@ -1112,11 +1139,17 @@ __global__ __launch_bounds__(kWg) void k_kv_join(KvAttendArgs a) {
   }
 }
 
-// Segments wanted: as many workgroups as the registers let the 256 CUs hold at once.
+// Workgroups of four waves that the registers let the 256 CUs hold at once: segments wanted.
 int attend_want(const KvCache& c) { return c.hd >= 256 ? 512 : c.hd == 128 ? 768 : 1024; }
-bool attend_splits(const KvCache& c, int rows, int heads) {
-  const int64_t n = (int64_t)rows * c.kv_heads * ((heads / c.kv_heads + 15) / 16);
-  return rows <= 256 && n <= attend_want(c) / 2 && c.max_pages > kMinHalves;
+int64_t attend_items(const KvCache& c, int rows, int heads) {
+  return (int64_t)rows * c.kv_heads * ((heads / c.kv_heads + 15) / 16);
+}
+// Rows are cut where they are few and may be long: what one workgroup walks in
+// the time of a join and its launch (32 half pages, or 256 KiB where they are wide) stays whole.
+bool attend_splits(const KvCache& c, int rows, int heads, int window) {
+  const int64_t most = std::min<int64_t>(2 * (int64_t)c.max_pages, window > 0 ? (int64_t)window / 32 + 2 : INT32_MAX);
+  const int64_t whole = std::min(kWholeHalves, (256 << 10) / kv_part_bytes(c.type, c.hd));
+  return rows <= 256 && attend_items(c, rows, heads) <= attend_want(c) / 2 && most > whole;
 }
 
 }  // namespace
@@ -1163,25 +1196,35 @@ hipError_t launch_kv_read(const KvReadArgs& a, hipStream_t s) {
 }
 
 int64_t kv_attend_floats(const KvCache& c, int rows, int heads) {
-  return attend_splits(c, rows, heads) ? (int64_t)attend_want(c) * std::min(heads / c.kv_heads, 16) * (c.hd + 2) : 0;
+  return attend_splits(c, rows, heads, 0) ? (int64_t)attend_want(c) * std::min(heads / c.kv_heads, 16) * (c.hd + 2) : 0;
 }
 
 hipError_t launch_kv_attend(const KvAttendArgs& a0, hipStream_t s) {
   KvAttendArgs a = a0;
-  const int G = a.heads / a.c.kv_heads, hgs = (G + 15) / 16, nh = std::min(G, 16);
-  a.split = attend_splits(a.c, a.rows, a.heads) ? 1 : 0;
+  const int G = a.heads / a.c.kv_heads, nh = std::min(G, 16);
+  const int64_t items = attend_items(a.c, a.rows, a.heads);
+  a.split = attend_splits(a.c, a.rows, a.heads, a.window) ? 1 : 0;
   a.want = attend_want(a.c);
   if (a.split && !a.part) return hipErrorInvalidValue;
-  const dim3 grid(a.split ? a.want : (uint32_t)((int64_t)a.rows * a.c.kv_heads * hgs));
-  const size_t sh = (size_t)4 * nh * (a.c.hd + 2) * 4;
-#define CHONK_KV_CASE(T, B, P)                                                                           \
-  if (a.c.type == T && a.c.hd == 32 * B && P == (nh <= 4)) {                                             \
+  const dim3 grid(a.split ? a.want : (uint32_t)items);
+  // whole rows of few workgroups: eight waves each, as long as all of them fit the CUs
+  const bool wide = !a.split && items <= (a.c.hd >= 128 ? 256 : 512);
+  const size_t sh = (size_t)(wide ? 8 : 4) * nh * (a.c.hd + 2) * 4;
+#define CHONK_KV_LAUNCH(T, B, P, W)                                                                      \
+  {                                                                                                      \
     if (sh > 32768) {                                                                                    \
-      const hipError_t e = hipFuncSetAttribute((const void*)k_kv_attend<T, B, P>,                        \
+      const hipError_t e = hipFuncSetAttribute((const void*)k_kv_attend<T, B, P, W>,                     \
                                                hipFuncAttributeMaxDynamicSharedMemorySize, (int)sh);     \
       if (e != hipSuccess) return e;                                                                     \
     }                                                                                                    \
-    hipLaunchKernelGGL((k_kv_attend<T, B, P>), grid, dim3(kWg), sh, s, a);                               \
+    hipLaunchKernelGGL((k_kv_attend<T, B, P, W>), grid, dim3(64 * W), sh, s, a);                         \
+  }
+#define CHONK_KV_CASE(T, B, P)                                                                           \
+  if (a.c.type == T && a.c.hd == 32 * B && P == (nh <= 4)) {                                             \
+    if (wide)                                                                                            \
+      CHONK_KV_LAUNCH(T, B, P, 8)                                                                        \
+    else                                                                                                 \
+      CHONK_KV_LAUNCH(T, B, P, 4)                                                                        \
   } else
 #define CHONK_KV_CASES(T, P) CHONK_KV_CASE(T, 1, P) CHONK_KV_CASE(T, 2, P) CHONK_KV_CASE(T, 4, P) CHONK_KV_CASE(T, 8, P)
   CHONK_KV_CASES(CHONK_KV_F16, false)
@@ -1193,6 +1236,7 @@ hipError_t launch_kv_attend(const KvAttendArgs& a0, hipStream_t s) {
   return hipErrorInvalidValue;
 #undef CHONK_KV_CASES
 #undef CHONK_KV_CASE
+#undef CHONK_KV_LAUNCH
   if (a.split) hipLaunchKernelGGL(k_kv_join, dim3(a.heads, a.rows), dim3(kWg), 0, s, a);
   return hipGetLastError();
 }
