@@ -66,6 +66,7 @@ __device__ __forceinline__ int place_of(int p) { return ((p & 15) >> 2) * 8 + (p
 
 typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
 typedef _Float16 h4u_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef _Float16 h8u_t __attribute__((ext_vector_type(8), aligned(2)));
 
 // Sums and maxima over the L lanes of a (row, head), without the LDS crossbar.
 template <int CTRL>
@@ -535,6 +536,9 @@ struct Codes {
         }
       }
     }
+  }
+  // (apart, and asked for first: the half page's work begins with them)
+  __device__ __forceinline__ void load_scales(const uint8_t* part, int u, int lane) {
     if constexpr (KV != CHONK_KV_F16) {
       const uint8_t* s = part + kv_code_bytes(KV, 32 * NB) + u * NB * 64;
       if constexpr (NB == 8) {
@@ -662,6 +666,29 @@ __device__ __forceinline__ Cut cut_rows(const KvAttendArgs& a, int items, F mine
              __builtin_amdgcn_readlane(c.segs, at)};
 }
 
+// The maximum over the 16 lanes of a row, a step an instruction. (Through the compiler a
+// step is a move, two quietings of NaNs and the maximum. A lane's value may not be
+// read across lanes for two cycles after it is written: hence the waits.)
+__device__ __forceinline__ float row_max(float v) {
+  asm("s_nop 1\n\tv_max_f32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n\t"
+      "s_nop 1\n\tv_max_f32_dpp %0, %0, %0 row_mirror row_mask:0xf bank_mask:0xf"
+      : "+v"(v));
+  return v;
+}
+// The larger of the two, and of the magnitudes of packed halves (their bits grow with them).
+__device__ __forceinline__ uint32_t top2(uint32_t a, uint32_t b) {
+  typedef unsigned short s2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s2_t, a), __builtin_bit_cast(s2_t, b)));
+}
+// fp16's exponent field of the largest of a lane's V scales (NaN and infinities as the largest
+// finite one): the scale is below 2^(field - 14)
+__device__ __forceinline__ float scale_field(uint32_t w) {
+  const uint32_t x = max(w & 0x7fffu, w >> 16 & 0x7fffu);
+  return (float)min(x >> 10, 30u);
+}
+
 // w * half H of d: the sum with 0 makes it one mixed instruction. (Not in asm: w
 // comes from an exponential, whose result the next instruction cannot take
 // without a wait that the compiler sees to.)
@@ -684,6 +711,12 @@ __device__ __forceinline__ float less_half(float w, uint32_t h) {
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
   lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(less_half<0>(x, hi), less_half<1>(y, hi)));
+}
+
+// Where a split call keeps each row's segments and its first one's workgroup: behind
+// the segments' rows and their (maximum, sum).
+__device__ __forceinline__ int* cuts(const KvAttendArgs& a, int nhm) {
+  return (int*)(a.part + (int64_t)a.want * nhm * (a.c.hd + 2));
 }
 
 // One workgroup per segment of a (row, kv head, up to 16 of its q heads); its
@@ -724,6 +757,11 @@ __global__ __launch_bounds__(64 * NW, NB == 8 ? 2 : NB == 4 ? (NW == 8 ? 2 : 3) 
     r = c.row, seq = c.seq, len = c.len, segs = c.segs;
     it = (id - c.before * items) / segs;
     seg = (id - c.before * items) % segs;
+    if (it == 0 && seg == 0 && tid == 0) {  // for the join
+      int* cut = cuts(a, min(G, 16)) + 2 * r;
+      cut[0] = seq < 0 ? 1 : segs;
+      cut[1] = id;
+    }
   } else {
     r = blockIdx.x / items;
     it = blockIdx.x % items;
@@ -732,31 +770,63 @@ __global__ __launch_bounds__(64 * NW, NB == 8 ? 2 : NB == 4 ? (NW == 8 ? 2 : 3) 
   }
   const int kv = it / hgs, hg = it % hgs;
   const int h0 = kv * G + hg * 16, nh = min(16, G - hg * 16);
+  // q on its way first (eight dims of each block, in their own order): it hangs on nothing
+  f4u_t qx[NB][2];
+  {
+    const int64_t o = r * a.q_ld + (int64_t)(h0 + min(PACK ? col & 3 : col, nh - 1)) * HD + 8 * g;
+    if (a.f16) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const h8u_t x = *(const h8u_t*)((const _Float16*)a.q + o + 32 * b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qx[b][e / 4][e & 3] = (float)x[e];
+      }
+    } else {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        qx[b][0] = *(const f4u_t*)((const float*)a.q + o + 32 * b);
+        qx[b][1] = *(const f4u_t*)((const float*)a.q + o + 32 * b + 4);
+      }
+    }
+  }
   const Span sp(a, seq, len, tid == 0);
   if (sp.seq < 0) return;  // (the join leaves the row alone too)
   const int per = (sp.h1 - sp.h0 + segs - 1) / segs;
   const int to = min(sp.h0 + (seg + 1) * per, sp.h1);
   int hx = sp.h0 + seg * per + wave;
 
-  // the first half page's K and V are on their way before anything else
+  // The first half page's K and V are on their way before anything else. The pages of
+  // the wave's next 64 half pages are one load, an id a lane.
   const int32_t* tab = a.c.table + (size_t)sp.seq * a.c.max_pages;
   const uint8_t* pool = a.c.pages + (size_t)kv * 2 * PART;
   const size_t page_bytes = (size_t)a.c.kv_heads * 2 * PART;
   bool poison = sp.bad;
-  auto part_of = [&](int h) {
-    int page = ld_scalar(tab + h / 2);
-    if (page < 0 || page >= a.c.n_pages) {
-      if (lane == 0) fault(a.c, KVF_PAGE);
-      poison = true;
-      page = 0;
+  int ids = 0, asked = 0;  // half pages asked for so far
+  const int hx0 = hx;
+  auto next_part = [&]() {
+    if ((asked & 63) == 0) {
+      const int h = hx0 + (asked + lane) * NW;
+      ids = h < to ? tab[h / 2] : 0;
+      const bool out = ids < 0 || ids >= a.c.n_pages;
+      if (__ballot(out)) {
+        if (out) fault(a.c, KVF_PAGE);
+        ids = out ? 0 : ids;
+        poison = true;
+      }
     }
-    return pool + (size_t)page * page_bytes;
+    return pool + (size_t)__builtin_amdgcn_readlane(ids, asked++ & 63) * page_bytes;
   };
   Codes<KV, NB> kc, vc;
+  const uint8_t* vnext = nullptr;  // ONE: where the V of K's half page is
   if (hx < to) {
-    const uint8_t* p = part_of(hx);
+    const uint8_t* p = next_part();
+    kc.load_scales(p, hx & 1, lane);
+    vc.load_scales(p + PART, hx & 1, lane);
     kc.load(p, hx & 1, lane);
-    if constexpr (!ONE) vc.load(p + PART, hx & 1, lane);
+    if constexpr (ONE)
+      vnext = p + PART;
+    else
+      vc.load(p + PART, hx & 1, lane);
   }
 
   // q: this lane's head at dims 32 b + 8 g + e, scaled by a power of two so that the
@@ -764,18 +834,11 @@ __global__ __launch_bounds__(64 * NW, NB == 8 ? 2 : NB == 4 ? (NW == 8 ? 2 : 3) 
   h8_t qr[QL ? 1 : NB][QP];
   float mul;             // score of S in powers of two
   {
-    float x[NB][8];
-    const int h = h0 + min(PACK ? col & 3 : col, nh - 1);
-    const int64_t o = r * a.q_ld + (int64_t)h * HD + 8 * g;
     float top = 0.f;
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int64_t at = o + 32 * b + kOrder<KV>(e);
-        x[b][e] = a.f16 ? (float)((const _Float16*)a.q)[at] : ((const float*)a.q)[at];
-        top = fmaxf(top, fabsf(x[b][e]));
-      }
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(qx[b][e / 4][e & 3]));
     float t0, t1;
     swap16(top, t0, t1);
     top = fmaxf(t0, t1);
@@ -791,7 +854,8 @@ __global__ __launch_bounds__(64 * NW, NB == 8 ? 2 : NB == 4 ? (NW == 8 ? 2 : 3) 
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float part = KV == CHONK_KV_Q4 && e >= 4 ? 0.0625f : 1.f;  // (high nibbles are 16 times their code)
-        const float y = x[b][e] * f * part;
+        const int k = kOrder<KV>(e);
+        const float y = qx[b][k / 4][k & 3] * f * part;
         hi[e] = (_Float16)y;
         lo[e] = (_Float16)(y - (float)hi[e]);
       }
@@ -815,11 +879,10 @@ __global__ __launch_bounds__(64 * NW, NB == 8 ? 2 : NB == 4 ? (NW == 8 ? 2 : 3) 
   const int pa = F ? 2 * pc : 8 * (pc >> 2) + (pc & 1) + 4 * ((pc >> 1) & 1), pb = pa + (F ? 1 : 2);
   if constexpr (PACK) mul = __shfl(mul, hc);
 
-  // m is the reference of the exponents: the running maximum mx less an offset that
-  // keeps weight * V scale below 2^14 and its bits above fp16's denormals; dtop is the largest
-  // exponent of a V scale so far
-  float mx = -1e30f, m = -1e30f, l = 0.f;
-  int dtop = 0;
+  // m is the reference of the exponents: the running maximum of score (in powers of
+  // two) and V scale together, less what keeps weight * scale below 2^14 and its
+  // bits above fp16's denormals. (A field is 0 at least, so no weight is above 2^29.)
+  float m = -1e30f, l = 0.f;
   f4_t acc[2 * NB];
 #pragma unroll
   for (int i = 0; i < 2 * NB; ++i) acc[i] = f4_t{0.f, 0.f, 0.f, 0.f};
@@ -828,6 +891,7 @@ __global__ __launch_bounds__(64 * NW, NB == 8 ? 2 : NB == 4 ? (NW == 8 ? 2 : 3) 
     const int j0 = 32 * hx;
     const bool edge = j0 < sp.first || j0 + 32 > sp.len;
     const bool more = hx + NW < to;
+    const uint8_t* next = nullptr;
     if constexpr (!F) {
       constexpr int D = NB == 8 ? 2 : 1;
       if (edge) {  // scales of unseen places may be anything
@@ -897,11 +961,14 @@ __global__ __launch_bounds__(64 * NW, NB == 8 ? 2 : NB == 4 ? (NW == 8 ? 2 : 3) 
       }
     }
     // (an even number of halves on: the same half of its page)
-    const uint8_t* next = ONE ? part_of(hx) : more ? part_of(hx + NW) : nullptr;
-    if constexpr (ONE)
-      vc.load(next + PART, hx & 1, lane);
-    else if (more)
+    if constexpr (ONE) {
+      vc.load(vnext, hx & 1, lane);
+    } else if (more) {
+      next = next_part();
+      kc.load_scales(next, hx & 1, lane);
+      vc.load_scales(next + PART, hx & 1, lane);
       kc.load(next, hx & 1, lane);
+    }
     if (edge) {
       uint32_t out = 0;
 #pragma unroll
@@ -919,19 +986,8 @@ __global__ __launch_bounds__(64 * NW, NB == 8 ? 2 : NB == 4 ? (NW == 8 ? 2 : 3) 
         for (int i = 0; i < NB * 8; ++i) vc.w[i] &= seen[i & 3];
       }
     }
-    float off = 14.f;
-    if constexpr (!F) {
-      uint32_t x = 0;
-#pragma unroll
-      for (int i = 0; i < (NB == 8 ? 2 : 1); ++i) {
-        const uint32_t lo = vc.d[i] & 0x7fffu, hi = vc.d[i] >> 16 & 0x7fffu;
-        x = max(x, max(lo > 0x7bffu ? 0 : lo, hi > 0x7bffu ? 0 : hi));
-      }
-      x = (uint32_t)wave_max((float)x);
-      dtop = max(dtop, (int)__builtin_amdgcn_readfirstlane(x) >> 10);
-      off = (float)(28 - dtop);
-    }
     float s0 = 0.f, s1 = 0.f, top;
+    uint32_t dv[NB];
     if constexpr (PACK) {
       if (col < 8) {
         *(float4*)(ss[wave] + col * 32 + 8 * g) = make_float4(s[0], s[1], s[2], s[3]);
@@ -941,17 +997,35 @@ __global__ __launch_bounds__(64 * NW, NB == 8 ? 2 : NB == 4 ? (NW == 8 ? 2 : 3) 
       __builtin_amdgcn_wave_barrier();
       s0 = ss[wave][hc * 32 + pa] + ss[wave][(hc + 4) * 32 + pa];
       s1 = ss[wave][hc * 32 + pb] + ss[wave][(hc + 4) * 32 + pb];
-      top = group_max<16>(fmaxf(s0, s1));
+      top = fmaxf(s0, s1) * mul;
+      if constexpr (!F) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) dv[b] = scv[wave][pc * NB + b];
+        uint32_t x = dv[0] & 0x7fff7fffu;
+#pragma unroll
+        for (int b = 1; b < NB; ++b) x = top2(x, dv[b] & 0x7fff7fffu);
+        top += scale_field(x);
+      }
+      top = row_max(top);
     } else {
-      top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+      top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))) * mul;
+      if constexpr (!F) {
+        uint32_t x = 0;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const uint4 d = *(const uint4*)(scv[wave] + b * 16 + g * 4);
+          x = top2(x, top2(top2(d.x & 0x7fff7fffu, d.y & 0x7fff7fffu), top2(d.z & 0x7fff7fffu, d.w & 0x7fff7fffu)));
+        }
+        top += scale_field(x);
+      }
       float t0, t1;
       swap16(top, t0, t1);
       top = fmaxf(t0, t1);
       swap32(top, t0, t1);
       top = fmaxf(t0, t1);
     }
-    mx = fmaxf(mx, top * mul);
-    const float ref = mx - off;
+    // weight < 2^14, or weight * scale < 2^(28 - field + field - 14)
+    const float ref = fmaxf(m, top - (F ? 14.f : 28.f));
     if (__ballot(ref != m)) {
       const float f = __builtin_amdgcn_exp2f(m - ref);
       l *= f;
@@ -965,11 +1039,6 @@ __global__ __launch_bounds__(64 * NW, NB == 8 ? 2 : NB == 4 ? (NW == 8 ? 2 : 3) 
       p[0] = __builtin_amdgcn_exp2f(fmaf(s0, mul, -m));
       p[1] = __builtin_amdgcn_exp2f(fmaf(s1, mul, -m));
       l += p[0] + p[1];
-      uint32_t dv[NB];
-      if constexpr (!F) {
-#pragma unroll
-        for (int b = 0; b < NB; ++b) dv[b] = scv[wave][pc * NB + b];
-      }
 #pragma unroll
       for (int b = 0; b < WB; ++b) {
         uint32_t hi, lo;
@@ -1017,7 +1086,11 @@ __global__ __launch_bounds__(64 * NW, NB == 8 ? 2 : NB == 4 ? (NW == 8 ? 2 : 3) 
       acc[2 * b + 1] = mfma(v1, wh, acc[2 * b + 1]);
     }
     if constexpr (ONE) {
-      if (more) kc.load(part_of(hx + NW), hx & 1, lane);
+      if (more) {
+        next = next_part();
+        kc.load(next, hx & 1, lane);
+        vnext = next + PART;
+      }
     } else if (more) {
       vc.load(next + PART, hx & 1, lane);
     }
@@ -1092,13 +1165,13 @@ __global__ __launch_bounds__(kWg) void k_kv_join(KvAttendArgs a) {
   __shared__ float wt[kMostWgs];
   __shared__ float red[8];
   __shared__ __align__(16) float so[kWg * 4];
-  const int G = a.heads / a.c.kv_heads, hgs = (G + 15) / 16, items = a.c.kv_heads * hgs, nhm = min(G, 16);
+  const int G = a.heads / a.c.kv_heads, hgs = (G + 15) / 16, nhm = min(G, 16);
   const int h = blockIdx.x, r = blockIdx.y, hd = a.c.hd, tid = threadIdx.x;
-  const Cut cut = cut_rows(a, items, [&](int t, int, int) { return t == r; });
-  const int segs = cut.segs;
-  if (segs == 1 || cut.seq < 0) return;
+  const int* cut = cuts(a, nhm) + 2 * r;
+  const int segs = ld_scalar(cut), slot = ld_scalar(cut + 1);
+  if (segs == 1) return;
   const int it = h / G * hgs + h % G / 16, hh = h % G % 16;
-  const int slot0 = cut.before * items + it * segs;
+  const int slot0 = slot + it * segs;
   const float* rows = a.part + ((int64_t)slot0 * nhm + hh) * hd;
   const float* ml = a.part + (int64_t)a.want * nhm * hd + ((int64_t)slot0 * nhm + hh) * 2;
   float M = -1e30f;
@@ -1196,7 +1269,7 @@ hipError_t launch_kv_read(const KvReadArgs& a, hipStream_t s) {
 }
 
 int64_t kv_attend_floats(const KvCache& c, int rows, int heads) {
-  return attend_splits(c, rows, heads, 0) ? (int64_t)attend_want(c) * std::min(heads / c.kv_heads, 16) * (c.hd + 2) : 0;
+  return attend_splits(c, rows, heads, 0) ? (int64_t)attend_want(c) * std::min(heads / c.kv_heads, 16) * (c.hd + 2) + 2 * rows : 0;
 }
 
 hipError_t launch_kv_attend(const KvAttendArgs& a0, hipStream_t s) {
