@@ -87,6 +87,14 @@ __device__ __forceinline__ double lanes_sum(double v) {
   return v;
 }
 
+// a / b from r = 1 / b rounded once: the quotient's error, exact in one fused step, times r
+// puts it right, as a division would round it (Markstein; b and the quotient are
+// far from the ends of fp32's range, or the quotient does not matter).
+__device__ __forceinline__ float quotient(float a, float b, float r) {
+  const float q = a * r;
+  return fmaf(fmaf(-q, b, a), r, q);
+}
+
 // Codes and scale of eight lanes' 32 values, four consecutive dims a lane. A
 // scale is the fp16 nearest to the exact one, and the codes count in units of
 // that fp16 number, so a code is off by at most half a unit of what is stored.
@@ -110,13 +118,13 @@ __device__ __forceinline__ uint32_t quantise(const float (&y)[4], int (&c)[4]) {
   step(dpp<0x4e>(m), 2);
   step(dpp<0x141>(m), 4);  // (the other four's: a mirrored row of eight)
   bad = fabsf(m) == INFINITY;
-  float d = KV == CHONK_KV_Q8 ? __fdiv_rn(fabsf(m), 127.f) : m * -0.125f;
+  float d = KV == CHONK_KV_Q8 ? quotient(fabsf(m), 127.f, 1.f / 127.f) : m * -0.125f;
   d = fminf(fmaxf(d, -65504.f), 65504.f);
   const _Float16 h = (_Float16)d;
-  const float dh = (float)h;
+  const float dh = (float)h, rh = __fdiv_rn(1.f, dh);
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    c[i] = bad || dh == 0.f ? 0 : (int)fminf(fmaxf(rintf(__fdiv_rn(y[i], dh)), kLow), kTop);
+    c[i] = bad || dh == 0.f ? 0 : (int)fminf(fmaxf(rintf(quotient(y[i], dh, rh)), kLow), kTop);
   return bad ? 0x7e00u : (uint32_t)__builtin_bit_cast(unsigned short, h);
 }
 
@@ -240,7 +248,7 @@ __global__ __launch_bounds__(kWg) void k_kv_append(KvAppendArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) sq += (double)y[i] * (double)y[i];
     sq = lanes_sum<L>(sq);
-    const float inv = (float)(1.0 / sqrt(sq / HD + a.eps));
+    const float inv = (float)rsqrt(sq * (1.0 / HD) + a.eps);
     y[0] = y[0] * inv * wt.x;
     y[1] = y[1] * inv * wt.y;
     y[2] = y[2] * inv * wt.z;
@@ -292,12 +300,10 @@ __global__ __launch_bounds__(kWg) void k_kv_append(KvAppendArgs a) {
 
 // ---- reading back -----------------------------------------------------------------
 
-// One thread per (row, kv head, eight dims): rows anywhere.
+// Eight dims of a row's place in `page`.
 template <int KV, bool F16>
-__device__ __forceinline__ void read8(const KvReadArgs& a, int r, int kv, int d0, int seq, int pos) {
+__device__ __forceinline__ void read8(const KvReadArgs& a, int r, int kv, int d0, int page, int pos) {
   const int hd = a.c.hd;
-  const int page = page_of(a.c, seq, pos, d0 == 0);
-  if (page < 0) return;
   const int part = kv_part_bytes(KV, hd), j = pos & (kKvPage - 1), p = j & 31, pl = place_of(p);
   const int unit = (j / 32) * (hd / 32) + d0 / 32, i0 = d0 & 31;
   const uint8_t* base = a.c.pages + ((size_t)page * a.c.kv_heads + kv) * 2 * part;
@@ -369,13 +375,12 @@ __global__ __launch_bounds__(kWg) void k_kv_read(KvReadArgs a) {
   const int s0 = __builtin_amdgcn_readlane(seq, first), p0 = __builtin_amdgcn_readlane(pos, first) - first;
   const bool odd = in && (seq != s0 || pos != p0 + (lane & 31));
   if (__ballot(odd) || (p0 & 31) || p0 < 0 || s0 < 0) {
-    // four lanes a row: its eight-dim runs of this block
-    for (int i = 0; i < 2; ++i) {
-      const int rr = r0 + 16 * i + (lane >> 2);
-      if (rr < 0 || rr >= a.rows) continue;
-      const int s = a.at.seq ? a.at.seq[rr] : a.at.seq0, p = a.at.pos ? a.at.pos[rr] : a.at.p0 + rr;
-      if (s >= 0) read8<KV, F16>(a, rr, kv, 32 * b + 8 * (lane & 3), s, p);
-    }
+    // two lanes a row, 16 of the block's dims each
+    if (!in || seq < 0) return;
+    const int page = page_of(a.c, seq, pos, it == 0 && lane < 32);
+    if (page < 0) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) read8<KV, F16>(a, r, kv, 32 * b + 16 * (lane >> 5) + 8 * i, page, pos);
     return;
   }
   const int page = page_of(a.c, s0, p0, lane == 0);
@@ -731,7 +736,7 @@ __device__ __forceinline__ int* cuts(const KvAttendArgs& a, int nhm) {
 // x 32 positions, go through LDS to two a lane, and the split weights back. Half the
 // products and a third fewer vector instructions.
 template <int KV, int NB, bool PACK, int NW>
-__global__ __launch_bounds__(64 * NW, NB == 8 ? 2 : NB == 4 ? (NW == 8 ? 2 : 3) : 4) void k_kv_attend(KvAttendArgs a) {
+__global__ __launch_bounds__(64 * NW, NB == 8 || (NB == 4 && (NW == 8 || (KV == CHONK_KV_F16 && !PACK))) ? 2 : NB == 4 ? 3 : 4) void k_kv_attend(KvAttendArgs a) {
   constexpr int HD = 32 * NB, PART = kv_part_bytes(KV, HD), WG = 64 * NW;
   constexpr bool F = KV == CHONK_KV_F16;
   constexpr int WB = F ? 1 : NB;            // blocks with weights of their own

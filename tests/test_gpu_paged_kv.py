@@ -273,6 +273,102 @@ def test_sizes_of_values_and_half_precision_rows(kv):
                 assert np.all((np.abs(got - want) <= tol)[fine]), float((np.abs(got - want) / tol)[fine].max())
 
 
+@pytest.mark.parametrize("kv", ref.TYPES)
+@pytest.mark.parametrize("heads,kv_heads,hd", [(16, 1, 256), (9, 1, 256), (5, 1, 128), (8, 8, 32), (32, 2, 64)])
+@pytest.mark.parametrize("max_pages", [1, 70])
+def test_attend_wide_groups_whole_and_split(kv, heads, kv_heads, hd, max_pages):
+    """Five to sixteen heads over one kv head, rows walked whole by eight waves and cut."""
+    c = Cache(kv, kv_heads, hd, n_seqs=2, max_pages=max_pages, seed=heads)
+    lengths = [1, 40, 64] if max_pages == 1 else [4480, 0, 2013]
+    seqs = np.array([0, 1, 1], np.int32)
+    q = c.rng.standard_normal((3, heads, hd)).astype(np.float32) * (1 if kv == "f16" else 4)
+    out = host(c.op.attend(dev(q), dev(seqs), dev(np.array(lengths, np.int32))))
+    c.op.check()
+    for r, n in enumerate(lengths):
+        k, v = c.stored(seqs[r], np.arange(n)) if n else (np.zeros((0, kv_heads, hd)),) * 2
+        want, mass, reach = ref.attend(q[r].astype(np.float64), k, v, hd ** -0.5)
+        tol = attend_tolerance(mass, reach, n, hd, 0.0)
+        assert np.all(np.abs(out[r] - want) <= tol), (n, float((np.abs(out[r] - want) / tol).max()))
+
+
+@pytest.mark.parametrize("rows", [255, 256, 257, 600])
+def test_many_rows_share_few_sequences(rows):
+    """Around the number of rows up to which they are cut; every row its own length, one of
+    16 empty and one of 16 left out, results equal to those of a call a row."""
+    c = Cache("q8", 1, 64, n_seqs=3, max_pages=40, seed=rows)
+    rng = c.rng
+    q = dev(rng.standard_normal((rows, 2, 64)).astype(np.float32))
+    seqs = rng.integers(0, 3, rows).astype(np.int32)
+    lengths = rng.integers(1, 2561, rows).astype(np.int32)
+    lengths[::16] = 0
+    seqs[5::16] = -1
+    out = torch.full_like(q, 9.0)
+    c.op.attend(q, dev(seqs), dev(lengths), out=out)
+    c.op.check()
+    out = host(out)
+    assert (out[5::16] == 9.0).all() and (out[::16] == 0.0).all()
+    k, v = zip(*(c.stored(s, np.arange(2560)) for s in range(3)))
+    for r in list(range(0, rows, 41)) + [rows - 1]:
+        if seqs[r] < 0 or lengths[r] == 0:
+            continue
+        n = lengths[r]
+        want, mass, reach = ref.attend(host(q)[r].astype(np.float64), k[seqs[r]][:n], v[seqs[r]][:n], 0.125)
+        tol = attend_tolerance(mass, reach, n, 64, 0.0)
+        assert np.all(np.abs(out[r] - want) <= tol), (r, float((np.abs(out[r] - want) / tol).max()))
+
+
+def test_two_streams_and_two_graphs_of_one_cache():
+    """Split calls of one cache on two streams at once, and two captured calls replayed together:
+    each has a workspace of its own."""
+    c = Cache("q4", 2, 128, n_seqs=1, max_pages=100, seed=8)
+    rng = c.rng
+    qs = [dev(rng.standard_normal((1, 32, 128)).astype(np.float32)) for _ in range(2)]
+    seqs, lengths = dev(np.zeros(1, np.int32)), [dev(np.array([n], np.int32)) for n in (6400, 5003)]
+    want = [c.op.attend(q, seqs, n).clone() for q, n in zip(qs, lengths)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(c.op.attend(qs[i], seqs, lengths[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+    graphs, outs = [], []
+    for i, s in enumerate(streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            outs.append(c.op.attend(qs[i], seqs, lengths[i]))
+        graphs.append(g)
+    for k in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(outs[i], want[i]) for i in range(2)), k
+        (qs[0] * 2).sum().item()
+
+
+@pytest.mark.parametrize("kv", ref.TYPES)
+def test_read_rows_in_any_order(kv):
+    """Whole half pages, ragged ends, rows out of order, the same row twice, another sequence's
+    rows between, rows left out: values do not depend on the company."""
+    c = Cache(kv, 3, 64, n_seqs=3, max_pages=4, seed=77)
+    runs = [(0, 0, 64), (1, 5, 100), (2, 40, 41), (0, 250, 256), (1, 31, 33), (2, 96, 160)]
+    seqs = np.concatenate([np.full(b - a, s) for s, a, b in runs] + [[0, 0, 2, 1], np.full(9, -1)]).astype(np.int32)
+    pos = np.concatenate([np.arange(a, b) for _, a, b in runs] + [[7, 7, 255, 0], np.arange(9)]).astype(np.int32)
+    for cut in (0, 1, 17, 70):  # where the first half page starts
+        s, p = seqs[cut:], pos[cut:]
+        for dtype in (torch.float16, torch.float32):
+            k, v = (host(x) for x in c.op.read(dev(s), dev(p), dtype))
+            for i in range(len(s) - 9):
+                want = c.stored(s[i], [p[i]])
+                kind = np.float16 if dtype == torch.float16 else np.float32
+                assert np.array_equal(k[i], want[0][0].astype(kind)) and np.array_equal(v[i], want[1][0].astype(kind)), (cut, i)
+    c.op.check()
+
+
 def test_rows_that_name_no_place():
     c = Cache("q8", 2, 64, n_seqs=2, max_pages=2)
     before = host(c.pages).copy()
