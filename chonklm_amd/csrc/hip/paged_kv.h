@@ -36,11 +36,11 @@ struct KvPlace {
 struct KvAppendArgs {
   KvCache c;
   KvPlace at;
-  PartSum q, k, v;        // fp32 rows (K-split partial sums); q.p null: k and v alone
-  const _Float16 *q16, *k16, *v16;  // fp16 rows instead (ld from the sums' ld)
-  void* q_out;            // rows of the input's type, q_ld elements apart
-  int64_t q_ld, k_ld, v_ld, qo_ld;
-  int32_t rows, heads, f16, vec;    // vec: every row is 16-byte aligned
+  PartSum q, k, v;        // fp32 rows (K-split partial sums, their ld not read); q.p null: k and v alone
+  const _Float16 *q16, *k16, *v16;  // fp16 rows instead
+  void* q_out;            // rows of the input's type
+  int64_t q_ld, k_ld, v_ld, qo_ld;  // elements from row to row
+  int32_t rows, heads, f16;
   const float *qn_w, *kn_w;
   double eps;
   const float2* rope;     // [rope_n][rope_dim / 2], or null

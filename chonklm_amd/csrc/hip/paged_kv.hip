@@ -335,29 +335,30 @@ __device__ __forceinline__ void read8(const KvReadArgs& a, int r, int kv, int d0
     if (!out) continue;
     const uint8_t* src = base + is_v * part;
     float x[8];
+    const int nk = k_piece(p, i0), nv = v_piece(p, i0);
     if constexpr (KV == CHONK_KV_F16) {
       const _Float16* h = (const _Float16*)src + (size_t)unit * 1024;
+      const h8_t k = __builtin_bit_cast(h8_t, ldg4(h + (p >> 4) * 512 + nk * 8));
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        x[i] = is_v ? (float)h[(i0 >> 4) * 512 + ((pl >> 3) * 16 + (i0 & 15) + i) * 8 + (pl & 7)]
-                    : (float)h[(p >> 4) * 512 + ((i0 >> 3) * 16 + (p & 15)) * 8 + i];
+      for (int i = 0; i < 8; ++i) x[i] = (float)(is_v ? h[(i0 >> 4) * 512 + (nv + i) * 8 + (pl & 7)] : k[i]);
     } else {
       const float d = h2f(((const uint16_t*)(src + kv_code_bytes(KV, hd)))[unit * 32 + pl]);
+      uint32_t c[8];
+      if constexpr (KV == CHONK_KV_Q8) {
+        const uint8_t* q = src + (size_t)unit * 1024;
+        const uint2 k = ldg2(q + nk * 16 + (p >> 4) * 8);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        int c;
-        if constexpr (KV == CHONK_KV_Q8) {
-          const uint8_t* q = src + (size_t)unit * 1024;
-          c = (is_v ? q[((pl >> 3) * 16 + (i0 & 15) + i) * 16 + (i0 >> 4) * 8 + (pl & 7)]
-                    : q[((i0 >> 3) * 16 + (p & 15)) * 16 + (p >> 4) * 8 + i]) - 128;
-        } else {
-          const uint8_t* q = src + (size_t)unit * 512;
-          const int byte = is_v ? q[((pl >> 3) * 16 + (i0 & 15) + i) * 8 + (pl & 7)]
-                                : q[((i0 >> 3) * 16 + (p & 15)) * 8 + (p >> 4) * 4 + (i & 3)];
-          c = ((is_v ? i0 >> 4 : i >> 2) ? byte >> 4 : byte & 15) - 8;
-        }
-        x[i] = (float)c * d;
+        for (int i = 0; i < 8; ++i)
+          c[i] = is_v ? q[(nv + i) * 16 + (i0 >> 4) * 8 + (pl & 7)] : (i < 4 ? k.x : k.y) >> (8 * (i & 3)) & 255;
+      } else {
+        const uint8_t* q = src + (size_t)unit * 512;
+        const uint32_t k = ldg1(q + nk * 8 + (p >> 4) * 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          c[i] = is_v ? q[(nv + i) * 8 + (pl & 7)] >> (i0 >> 4 ? 4 : 0) & 15 : k >> (8 * (i & 3) + 4 * (i >> 2)) & 15;
       }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = (float)((int)c[i] - (KV == CHONK_KV_Q8 ? 128 : 8)) * d;
     }
     if constexpr (F16) {
 #pragma unroll
@@ -383,8 +384,7 @@ __global__ __launch_bounds__(kWg) void k_kv_read(KvReadArgs a) {
   const int shift = (a.at.pos ? a.at.pos[0] : a.at.p0) & 31;
   const int groups = (a.rows + shift + 31) / 32;
   // (kv heads and blocks before rows: a row's pieces are written close in time)
-  const int64_t task = (int64_t)blockIdx.x * 4 + wave;
-  const int per = a.c.kv_heads * nb;
+  const uint32_t task = blockIdx.x * 4 + wave, per = (uint32_t)(a.c.kv_heads * nb);
   const int grp = (int)(task / per), it = (int)(task % per), kv = it / nb, b = it % nb;
   if (grp >= groups) return;
   const int r0 = grp * 32 - shift, r = r0 + (lane & 31);
@@ -1468,13 +1468,10 @@ int chonk_kv_append(const chonk_kv_cache* cache, const chonk_kv_rows* rows, cons
       a.v16 = (const _Float16*)x->v;
     } else {
       const void* src[3] = {x->q, x->k, x->v};
-      const int64_t ld[3] = {x->q_stride, x->k_stride, x->v_stride};
       PartSum* dst[3] = {&a.q, &a.k, &a.v};
       for (int i = 0; i < 3; ++i) {
-        if (ld[i] > INT32_MAX) throw Error(CHONK_EINVAL, "paged K/V cache: rows are too far apart");
         dst[i]->p = (const float*)src[i];
         dst[i]->ks = 1;
-        dst[i]->ld = (int32_t)ld[i];
       }
     }
     a.qn_w = x->q_norm;

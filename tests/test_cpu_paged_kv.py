@@ -3,6 +3,9 @@
 from __future__ import annotations
 
 import ctypes as C
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -116,3 +119,32 @@ def test_reference_quantiser_is_within_half_a_unit():
         c = np.clip(np.rint(x / d), -127 if kv == "q8" else -8, 127 if kv == "q8" else 7)
         ok = np.abs(x / d) <= (127 if kv == "q8" else 7.5)
         assert (np.abs(c * d - x) <= np.abs(d) * 0.5 * (1 + 1e-9) + 1e-12)[ok].all()
+
+
+def test_torch_after_the_library_is_refused():
+    """libchonk.so loaded before torch runs on another HIP runtime than torch's tensors and streams."""
+    code = ("from chonklm_amd._lib import lib\nlib()\nfrom chonklm_amd.paged_kv import ChonkError, PagedKv\n"
+            "try:\n    PagedKv(None, None, 2, 64)\nexcept ChonkError as e:\n    print('refused:', e)\n")
+    root = Path(__file__).resolve().parents[1]
+    out = subprocess.run([sys.executable, "-c", code], cwd=root, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
+    assert "refused: paged K/V cache: libchonk.so was loaded before torch" in out.stdout, out.stdout + out.stderr
+
+
+def test_tensors_off_the_gpu_are_refused():
+    import torch
+
+    from chonklm_amd.paged_kv import ChonkError, PagedKv, page_bytes
+
+    pages = torch.zeros((2, page_bytes("q4", 2, 64)), dtype=torch.uint8)
+    table = torch.zeros((1, 2), dtype=torch.int32)
+    for f, text in ((lambda: PagedKv(pages, table, 2, 64, "q4"), "must be on a GPU"),
+                    (lambda: PagedKv(pages, table, 2, 64, "q8"), "pages must be contiguous uint8"),
+                    (lambda: PagedKv(pages, table, 2, 64, "q5"), "unsupported kv type"),
+                    (lambda: PagedKv(pages, table, 2, 72, "q4"), "head_dim must be"),
+                    (lambda: PagedKv(pages, table.long(), 2, 64, "q4"), "table must be contiguous int32"),
+                    (lambda: page_bytes("f32", 2, 64), "unsupported kv type")):
+        with pytest.raises(ChonkError, match=text) as e:
+            f()
+        assert e.value.status_name == "EINVAL"
+    with pytest.raises(TypeError):
+        PagedKv(pages)

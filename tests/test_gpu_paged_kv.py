@@ -455,6 +455,39 @@ def test_steps_together_eager_and_captured(kv):
     a.op.check(), b.op.check()
 
 
+@pytest.mark.parametrize("kv", ref.TYPES)
+def test_pools_past_four_gigabytes(kv):
+    """Pages whose bytes lie past 2^32 of the pool (and past 2^31 before it)."""
+    size = page_bytes(kv, 8, 128)
+    n_pages = (9 << 29) // size + 3
+    pages = torch.empty((n_pages, size), dtype=torch.uint8, device=DEV)
+    ids = np.array([[n_pages - 1, (5 << 29) // size, 0]], np.int32)
+    op = PagedKv(pages, dev(ids), 8, 128, kv)
+    rng = np.random.default_rng(6)
+    k, v = (dev(rng.standard_normal((150, 8, 128)), torch.float32) for _ in range(2))
+    seqs, pos = dev(np.zeros(150, np.int32)), dev(np.arange(150, dtype=np.int32))
+    op.append(None, k, v, seqs, pos)
+    got_k, got_v = op.read(seqs, pos, torch.float32)
+    stored = ref.gather(kv, host(pages[dev(ids[0]).long()]), np.array([[0, 1, 2]]), 8, 128, 0, range(150))
+    assert np.array_equal(host(got_k), stored[0].astype(np.float32)) and np.array_equal(host(got_v), stored[1].astype(np.float32))
+    check_codes(kv, host(got_k).astype(np.float64), host(k).astype(np.float64), 0.0)
+    q = dev(rng.standard_normal((1, 16, 128)), torch.float32)
+    out = host(op.attend(q, seqs[:1], dev(np.array([150], np.int32))))
+    want, mass, reach = ref.attend(host(q)[0].astype(np.float64), *stored, 128 ** -0.5)
+    assert np.all(np.abs(out[0] - want) <= attend_tolerance(mass, reach, 150, 128, 0.0))
+
+
+def test_rows_that_want_a_gradient_are_refused():
+    c = Cache("q8", 2, 64, n_seqs=1, max_pages=1)
+    q, k = torch.ones((1, 4, 64), device=DEV, requires_grad=True), torch.ones((1, 2, 64), device=DEV)
+    i = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for f in (lambda: c.op.attend(q, i, i + 1), lambda: c.op.append(q, k, k, i, i)):
+        with pytest.raises(ChonkError, match="requires a gradient"):
+            f()
+        with torch.no_grad():
+            f()
+
+
 def test_refusals_of_tensors():
     c = Cache("q8", 2, 64, n_seqs=2, max_pages=2)
     q, k = torch.zeros((3, 4, 64), device=DEV), torch.zeros((3, 2, 64), device=DEV)
