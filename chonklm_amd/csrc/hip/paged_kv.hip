@@ -1238,17 +1238,20 @@ __global__ __launch_bounds__(kWg) void k_kv_join(KvAttendArgs a) {
   }
 }
 
-// Workgroups of four waves that the registers let the 256 CUs hold at once: segments wanted.
+// Workgroups of four waves that the registers let the 256 CUs hold at once: segments wanted
+// (more would wait for a place: 41k positions of 128 dims took 28 us in 1024, 22 in 768).
 int attend_want(const KvCache& c) { return c.hd >= 256 ? 512 : c.hd == 128 ? 768 : 1024; }
 int64_t attend_items(const KvCache& c, int rows, int heads) {
   return (int64_t)rows * c.kv_heads * ((heads / c.kv_heads + 15) / 16);
 }
-// Rows are cut where they are few and may be long: what one workgroup walks in
-// the time of a join and its launch (32 half pages, or 256 KiB where they are wide) stays whole.
+// Rows are cut where they are few and may be long: up to 32 half pages a row, one
+// workgroup walks them in the time of the shorter walk and its join. (24 x 12 rows of up to
+// 1024 positions of 64 dims in 8 bits: 11.7 us whole, 13.4 + 4.2 cut; 48 rows of 512
+// positions of 256 dims in fp16: 14.5 whole, 12.8 + 3.9 cut. 5 x 8 rows of 4094 positions
+// of 64 dims in 4 bits: 10 + 3.9 cut, 40 workgroups of 128 half pages whole.)
 bool attend_splits(const KvCache& c, int rows, int heads, int window) {
   const int64_t most = std::min<int64_t>(2 * (int64_t)c.max_pages, window > 0 ? (int64_t)window / 32 + 2 : INT32_MAX);
-  const int64_t whole = std::min(kWholeHalves, (256 << 10) / kv_part_bytes(c.type, c.hd));
-  return rows <= 256 && attend_items(c, rows, heads) <= attend_want(c) / 2 && most > whole;
+  return rows <= 256 && attend_items(c, rows, heads) <= attend_want(c) / 2 && most > kWholeHalves;
 }
 
 }  // namespace
@@ -1307,7 +1310,9 @@ hipError_t launch_kv_attend(const KvAttendArgs& a0, hipStream_t s) {
   a.want = attend_want(a.c);
   if (a.split && !a.part) return hipErrorInvalidValue;
   const dim3 grid(a.split ? a.want : (uint32_t)items);
-  // whole rows of few workgroups: eight waves each, as long as all of them fit the CUs
+  // whole rows of few workgroups: eight waves each, as long as all of them fit the CUs (3 rows
+  // of 301 positions of 64 dims: 5.2 us, 6.5 with four waves; 512 rows of up to 640 of 128
+  // dims need two rounds of the CUs with eight, and are walked in one, 13 us, with four)
   const bool wide = !a.split && items <= (a.c.hd >= 128 ? 256 : 512);
   const size_t sh = (size_t)(wide ? 8 : 4) * nh * (a.c.hd + 2) * 4;
 #define CHONK_KV_LAUNCH(T, B, P, W)                                                                      \
