@@ -64,7 +64,9 @@ struct KvAttendArgs {
   void* out;
   int64_t q_ld, o_ld;
   int32_t rows, heads, f16, window;
-  int32_t split, want;    // set by the launcher: rows are cut into at most `want` segments, joined from part
+  // set by the launcher: rows are cut into at most `want` segments, joined from part, unless the
+  // longest has at most `whole` half pages (many: or the rows are about as long as each other)
+  int32_t split, want, whole, many;
   float scale;
   float* part;
 };

@@ -31,9 +31,11 @@ typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
-constexpr int kMostWgs = 1024;  // segments of a split attention, at most
+constexpr int kMostWgs = 2048;  // segments of a split attention, at most
 constexpr int kWholeHalves = 32;  // half pages of a row that is never cut
-constexpr int kMinHalves = 8;   // ... of at least so many half pages
+// ... of at least so many half pages (5 x 8 rows of 4094 positions of 64 dims in 4 bits: 10.8 us in
+// segments of 8, 12.3 of 16; 48 rows of 512 of 256 dims in fp16: 12.8 of 8, 13.0 of 4)
+constexpr int kMinHalves = 8;
 
 __device__ __forceinline__ f4_t mfma(h8_t a, h8_t b, f4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -216,6 +218,9 @@ __device__ __forceinline__ void row4(const PartSum& P, const _Float16* p16, int6
 // Every product and sum after the norm's is rounded by itself (no fused multiply-add)
 // and the norm's sum of squares is taken in 64 bits: the codes do not depend on which
 // path (prompt rows or single tokens) wrote them.
+// Measured: 17.7 us for 2047 rows of 16 + 8 + 8 heads x 128 fp32 to 8 bits (34 MB read, 21 MB
+// written, 3.1 of the 4.7 TB/s that a large copy makes: V's codes leave a byte at a time), 4 to
+// 4.5 us for up to 64 rows, of which a launch and its dependent trips to memory are all.
 template <int KV, bool F16, int NB>
 __global__ __launch_bounds__(kWg) void k_kv_append(KvAppendArgs a) {
 #pragma clang fp contract(off)
@@ -378,6 +383,8 @@ __device__ __forceinline__ int byte_of(uint32_t w, int k) { return (int)(w >> (8
 // positions (what a prompt's and a history's are, but at its ends) are read in the pages' own
 // order, a unit of 1 KiB (8 bits) at a time, and leave in whole 64-byte pieces; others
 // one by one. The rows' groups start where row 0's half page does.
+// Bound by the bytes: 20 us for 11003 positions of 8 heads x 128 from 8 bits to fp32, 114 MB:
+// 5.7 TB/s (a large copy, which no cache holds, makes 4.7); 3 us for one row.
 template <int KV, bool F16>
 __global__ __launch_bounds__(kWg) void k_kv_read(KvReadArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hd = a.c.hd, nb = hd / 32;
@@ -618,11 +625,12 @@ struct Span {
   }
 };
 
-// The rows' cut into segments, the same in every wave: at most `want`
-// segments (at least kMinHalves long) of about as many halves each, found from all the rows' lengths, so that
+// The rows' cut into segments, the same in every wave: at most `want` segments (at least
+// kMinHalves long) of about as many halves each, found from all the rows' lengths, so that
 // ragged rows keep the device as evenly busy as equal ones and the host needs to know no
-// length. A lane looks at rows 4 lane .. 4 lane + 3 (at most 256 rows). The row that
-// `mine` holds for comes back in all lanes (row -1: none).
+// length. Rows none of which is long, and many of like length (the longest within 1.5 times the
+// mean), stay whole. A lane looks at rows 4 lane .. 4 lane + 3 (at most 256 rows). The row
+// that `mine` holds for comes back in all lanes (row -1: none).
 struct Cut {
   int row, seq, len, before, segs;  // segments of the rows before it (an item each), segments of its items
 };
@@ -645,14 +653,21 @@ __device__ __forceinline__ Cut cut_rows(const KvAttendArgs& a, int items, F mine
   // The shortest length of a segment that leaves at most `want` of them: between an
   // even share and what must do (every item's last segment may be short), by halving. As
   // floats: whatever the length, the segments it gives are the same in every wave.
-  float total = 0.f;
+  float total = 0.f, longest = 0.f;
 #pragma unroll
-  for (int i = 0; i < R; ++i) total += (float)n[i];
+  for (int i = 0; i < R; ++i) {
+    total += (float)n[i];
+    longest = fmaxf(longest, (float)n[i]);
+  }
   total = wave_sum(total) * (float)items;
+  longest = wave_max(longest);
   const float want = (float)a.want;
   float lo = total / want, hi = total / (want - (float)(a.rows * items)) * 1.0001f + 1.f;
   auto pieces = [&](int i, float most) { return r0 + i < a.rows ? max(1, (int)ceilf((float)n[i] / most)) : 0; };
-  if (hi > (float)kMinHalves) {
+  const bool whole = longest <= (float)a.whole || (a.many && longest * (float)(a.rows * items) <= 1.5f * total);
+  if (whole) {
+    hi = fmaxf(longest, 1.f);
+  } else if (hi > (float)kMinHalves) {
     for (int k = 0; k < 4; ++k) {
       const float mid = 0.5f * (lo + hi);
       int t = 0;
@@ -756,6 +771,11 @@ __device__ __forceinline__ int* cuts(const KvAttendArgs& a, int nhm) {
 // V's scales, their split) would be done on all 16, the scores of a half page, 4 heads
 // x 32 positions, go through LDS to two a lane, and the split weights back. Half the
 // products and a third fewer vector instructions.
+//
+// Bound by the pages' bytes where rows are long: 32 rows of up to 16k positions of 8 heads x 128 in
+// 4 bits take 67 us for 302 MB, 4.5 of the 4.7 TB/s that a large copy makes; one row of 41k in 8
+// bits 20 us for 89 MB, 4.4 TB/s. Short rows are bound by the chain of dependent trips to memory
+// (length, page id, K and V, for split rows the cut before it): 5.2 us for one of 301 x 3 heads x 64.
 template <int KV, int NB, bool PACK, int NW>
 __global__ __launch_bounds__(64 * NW, NB == 8 || (NB == 4 && (NW == 8 || (KV == CHONK_KV_F16 && !PACK))) ? 2 : NB == 4 ? 3 : 4) void k_kv_attend(KvAttendArgs a) {
   constexpr int HD = 32 * NB, PART = kv_part_bytes(KV, HD), WG = 64 * NW;
@@ -1186,7 +1206,9 @@ __global__ __launch_bounds__(64 * NW, NB == 8 || (NB == 4 && (NW == 8 || (KV == 
 }
 
 // Joins a (row, head)'s segments: HD / 4 columns of float4, the segments over
-// groups of threads, every group's in order and the groups in order.
+// groups of threads, every group's in order and the groups in order: the result does not
+// hang on which workgroup ended first. Bound by its launch and two trips to memory: 3.9 us for 5
+// rows of 16 heads x 64, 4.5 for 16 heads x 128 of one row in 96 segments each.
 __global__ __launch_bounds__(kWg) void k_kv_join(KvAttendArgs a) {
   __shared__ float wt[kMostWgs];
   __shared__ float red[8];
@@ -1238,27 +1260,39 @@ __global__ __launch_bounds__(kWg) void k_kv_join(KvAttendArgs a) {
   }
 }
 
-// Workgroups of four waves that the registers let the 256 CUs hold at once: segments wanted
-// (more would wait for a place: 41k positions of 128 dims took 28 us in 1024, 22 in 768).
-int attend_want(const KvCache& c) { return c.hd >= 256 ? 512 : c.hd == 128 ? 768 : 1024; }
 int64_t attend_items(const KvCache& c, int rows, int heads) {
   return (int64_t)rows * c.kv_heads * ((heads / c.kv_heads + 15) / 16);
 }
-// Rows are cut where they are few and may be long: up to 32 half pages a row, one
-// workgroup walks them in the time of the shorter walk and its join. (24 x 12 rows of up to
-// 1024 positions of 64 dims in 8 bits: 11.7 us whole, 13.4 + 4.2 cut; 48 rows of 512
-// positions of 256 dims in fp16: 14.5 whole, 12.8 + 3.9 cut. 5 x 8 rows of 4094 positions
-// of 64 dims in 4 bits: 10 + 3.9 cut, 40 workgroups of 128 half pages whole.)
+// Workgroups of four waves that the registers let the 256 CUs hold at once: segments wanted of
+// few (row, head)s (more would wait for a place: 41k positions of 128 dims took 28 us in
+// 1024, 22 in 768).
+int attend_once(const KvCache& c) { return c.hd >= 256 ? 512 : c.hd == 128 ? 768 : 1024; }
+bool attend_many(const KvCache& c, int64_t items) { return items > attend_once(c) / 2; }
+// Many of them, which fill half of the device or more as they are: twice that, two segments
+// for each at least.
+int attend_want(const KvCache& c, int64_t items) { return attend_once(c) * (attend_many(c, items) ? 2 : 1); }
+// Half pages up to which rows stay whole: one workgroup walks them in the time of the
+// shorter walk and its join. (24 x 12 rows of up to 1024 positions of 64 dims in 8 bits: 11.7 us
+// whole, 13.4 + 4.2 cut; 48 rows of 512 positions of 256 dims in fp16: 14.5 whole, 12.8 + 3.9
+// cut; 32 x 8 of 640 of 128 dims in 8 bits: 14.1 whole, 18.3 cut.) Many rows longer than that
+// share the device well unless their lengths differ (64 x 8 of 128 dims in 4 bits, of up to
+// 2048: 29.9 us whole, 34.4 cut; of 1 to 16384: 205 whole, 133 cut).
+int attend_whole(const KvCache& c, int64_t items) { return attend_many(c, items) ? 4 * kWholeHalves : kWholeHalves; }
+// Whether rows may be cut: the lengths are the device's to know (cut_rows), the table's
+// width is known here. (Rows that could have been cut and were not, 64 x 8 of 640: 16.5 us
+// instead of 13.7.)
 bool attend_splits(const KvCache& c, int rows, int heads, int window) {
   const int64_t most = std::min<int64_t>(2 * (int64_t)c.max_pages, window > 0 ? (int64_t)window / 32 + 2 : INT32_MAX);
-  return rows <= 256 && attend_items(c, rows, heads) <= attend_want(c) / 2 && most > kWholeHalves;
+  const int64_t items = attend_items(c, rows, heads);
+  return rows <= 256 && items <= attend_once(c) && most > attend_whole(c, items);
 }
 
 }  // namespace
 
 hipError_t launch_kv_append(const KvAppendArgs& a, hipStream_t s) {
   const int slots = ((a.f16 ? a.q16 != nullptr : a.q.p != nullptr) ? a.heads : 0) + 2 * a.c.kv_heads;
-  // as many ranges of slots as fill the device (1024 workgroups)
+  // as many ranges of slots as fill the device (2047 rows of 32 heads x 128: 18.6 us in 1024
+  // workgroups, 19.1 in 2048, whose rows are fetched again for every range)
   const int groups = (a.rows + kWg / (a.c.hd / 4) - 1) / (kWg / (a.c.hd / 4));
   const dim3 grid(groups, std::max(1, std::min(slots, 1024 / groups)));
 #define CHONK_KV_CASE(T, B)                                                                 \
@@ -1299,7 +1333,7 @@ hipError_t launch_kv_read(const KvReadArgs& a, hipStream_t s) {
 }
 
 int64_t kv_attend_floats(const KvCache& c, int rows, int heads) {
-  return attend_splits(c, rows, heads, 0) ? (int64_t)attend_want(c) * std::min(heads / c.kv_heads, 16) * (c.hd + 2) + 2 * rows : 0;
+  return attend_splits(c, rows, heads, 0) ? (int64_t)attend_want(c, attend_items(c, rows, heads)) * std::min(heads / c.kv_heads, 16) * (c.hd + 2) + 2 * rows : 0;
 }
 
 hipError_t launch_kv_attend(const KvAttendArgs& a0, hipStream_t s) {
@@ -1307,12 +1341,14 @@ hipError_t launch_kv_attend(const KvAttendArgs& a0, hipStream_t s) {
   const int G = a.heads / a.c.kv_heads, nh = std::min(G, 16);
   const int64_t items = attend_items(a.c, a.rows, a.heads);
   a.split = attend_splits(a.c, a.rows, a.heads, a.window) ? 1 : 0;
-  a.want = attend_want(a.c);
+  a.want = attend_want(a.c, items);
+  a.many = attend_many(a.c, items);
+  a.whole = attend_whole(a.c, items);
   if (a.split && !a.part) return hipErrorInvalidValue;
   const dim3 grid(a.split ? a.want : (uint32_t)items);
-  // whole rows of few workgroups: eight waves each, as long as all of them fit the CUs (3 rows
-  // of 301 positions of 64 dims: 5.2 us, 6.5 with four waves; 512 rows of up to 640 of 128
-  // dims need two rounds of the CUs with eight, and are walked in one, 13 us, with four)
+  // whole rows of few workgroups: eight waves each, as long as all of them fit the CUs (a row
+  // of 301 positions of 3 heads x 64: 5.2 us, 6.5 with four waves; 64 rows of up to 640 of 8 x
+  // 128 need two rounds of the CUs with eight, and are walked in one, 13 us, with four)
   const bool wide = !a.split && items <= (a.c.hd >= 128 ? 256 : 512);
   const size_t sh = (size_t)(wide ? 8 : 4) * nh * (a.c.hd + 2) * 4;
 #define CHONK_KV_LAUNCH(T, B, P, W)                                                                      \

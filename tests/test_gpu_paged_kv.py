@@ -317,6 +317,34 @@ def test_many_rows_share_few_sequences(rows):
         assert np.all(np.abs(out[r] - want) <= tol), (r, float((np.abs(out[r] - want) / tol).max()))
 
 
+@pytest.mark.parametrize("kv,rows,heads,kv_heads,hd", [("q8", 64, 12, 12, 64), ("q4", 64, 32, 8, 128), ("q4", 96, 8, 8, 128),
+                                                      ("q8", 97, 8, 8, 128), ("f16", 200, 4, 2, 256)])
+@pytest.mark.parametrize("lengths", ["ragged", "like", "short", "one long"])
+@pytest.mark.parametrize("window", [0, 4200])
+def test_many_rows_of_long_tables(kv, rows, heads, kv_heads, hd, lengths, window):
+    """Enough (row, head)s to fill half of the device: cut where the lengths differ, whole
+    where they are alike or short, or where there are more than the device holds at once."""
+    c = Cache(kv, kv_heads, hd, n_seqs=2, max_pages=70, seed=rows + hd)
+    rng = c.rng
+    q = dev(rng.standard_normal((rows, heads, hd)).astype(np.float32) * (1 if kv == "f16" else 4))
+    seqs = rng.integers(0, 2, rows).astype(np.int32)
+    n = {"ragged": rng.integers(1, 4481, rows), "like": rng.integers(4300, 4481, rows),
+         "short": rng.integers(1, 4097, rows), "one long": np.full(rows, 33)}[lengths].astype(np.int32)
+    n[rows // 2] = 4096 if lengths == "short" else 4480
+    n[3], seqs[7] = 0, -1
+    out = torch.full_like(q, 9.0)
+    c.op.attend(q, dev(seqs), dev(n), window=window, out=out)
+    c.op.check()
+    out = host(out)
+    assert np.isfinite(out).all() and (out[7] == 9.0).all() and (out[3] == 0.0).all()
+    k, v = zip(*(c.stored(s, np.arange(4480)) for s in range(2)))
+    for r in (0, rows // 2, int(n.argmax()), rows - 1):
+        at = slice(max(0, n[r] - window) if window else 0, n[r])
+        want, mass, reach = ref.attend(host(q)[r].astype(np.float64), k[seqs[r]][at], v[seqs[r]][at], hd ** -0.5)
+        tol = attend_tolerance(mass, reach, n[r], hd, 0.0)
+        assert np.all(np.abs(out[r] - want) <= tol), (r, float((np.abs(out[r] - want) / tol).max()))
+
+
 def test_two_streams_and_two_graphs_of_one_cache():
     """Split calls of one cache on two streams at once, and two captured calls replayed together:
     each has a workspace of its own."""
