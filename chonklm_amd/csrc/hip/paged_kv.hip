@@ -383,8 +383,9 @@ __device__ __forceinline__ int byte_of(uint32_t w, int k) { return (int)(w >> (8
 // positions (what a prompt's and a history's are, but at its ends) are read in the pages' own
 // order, a unit of 1 KiB (8 bits) at a time, and leave in whole 64-byte pieces; others
 // one by one. The rows' groups start where row 0's half page does.
-// Bound by the bytes: 20 us for 11003 positions of 8 heads x 128 from 8 bits to fp32, 114 MB:
-// 5.7 TB/s (a large copy, which no cache holds, makes 4.7); 3 us for one row.
+// Bound by the bytes: 25 to 27 us for 11003 positions of 8 heads x 128 from 8 bits to fp32, 114
+// MB, 4.2 to 4.5 TB/s (a large copy makes 4.7; 20 us where the last cache still holds the memory
+// that the results go to); 3 us for one row.
 template <int KV, bool F16>
 __global__ __launch_bounds__(kWg) void k_kv_read(KvReadArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hd = a.c.hd, nb = hd / 32;
