@@ -10,6 +10,8 @@ exponential's 2^-21; the weighted sum of n terms adds n 2^-24.
 """
 from __future__ import annotations
 
+import functools
+
 import numpy as np
 import pytest
 import torch
@@ -317,15 +319,22 @@ def test_many_rows_share_few_sequences(rows):
         assert np.all(np.abs(out[r] - want) <= tol), (r, float((np.abs(out[r] - want) / tol).max()))
 
 
-@pytest.mark.parametrize("kv,rows,heads,kv_heads,hd", [("q8", 64, 12, 12, 64), ("q4", 64, 32, 8, 128), ("q4", 96, 8, 8, 128),
-                                                      ("q8", 97, 8, 8, 128), ("f16", 200, 4, 2, 256)])
+@functools.lru_cache(maxsize=1)
+def _long_tables(kv, kv_heads, hd):
+    """A cache of two sequences of 4480 positions, and what they hold."""
+    c = Cache(kv, kv_heads, hd, n_seqs=2, max_pages=70, seed=hd)
+    return (c,) + tuple(zip(*(c.stored(s, np.arange(4480)) for s in range(2))))
+
+
 @pytest.mark.parametrize("lengths", ["ragged", "like", "short", "one long"])
 @pytest.mark.parametrize("window", [0, 4200])
+@pytest.mark.parametrize("kv,rows,heads,kv_heads,hd", [("q8", 64, 12, 12, 64), ("q4", 64, 32, 8, 128), ("q4", 96, 8, 8, 128),
+                                                      ("q8", 97, 8, 8, 128), ("f16", 200, 4, 2, 256)])
 def test_many_rows_of_long_tables(kv, rows, heads, kv_heads, hd, lengths, window):
     """Enough (row, head)s to fill half of the device: cut where the lengths differ, whole
     where they are alike or short, or where there are more than the device holds at once."""
-    c = Cache(kv, kv_heads, hd, n_seqs=2, max_pages=70, seed=rows + hd)
-    rng = c.rng
+    c, k, v = _long_tables(kv, kv_heads, hd)
+    rng = np.random.default_rng(rows)
     q = dev(rng.standard_normal((rows, heads, hd)).astype(np.float32) * (1 if kv == "f16" else 4))
     seqs = rng.integers(0, 2, rows).astype(np.int32)
     n = {"ragged": rng.integers(1, 4481, rows), "like": rng.integers(4300, 4481, rows),
@@ -337,7 +346,6 @@ def test_many_rows_of_long_tables(kv, rows, heads, kv_heads, hd, lengths, window
     c.op.check()
     out = host(out)
     assert np.isfinite(out).all() and (out[7] == 9.0).all() and (out[3] == 0.0).all()
-    k, v = zip(*(c.stored(s, np.arange(4480)) for s in range(2)))
     for r in (0, rows // 2, int(n.argmax()), rows - 1):
         at = slice(max(0, n[r] - window) if window else 0, n[r])
         want, mass, reach = ref.attend(host(q)[r].astype(np.float64), k[seqs[r]][at], v[seqs[r]][at], hd ** -0.5)
