@@ -817,7 +817,8 @@ __global__ __launch_bounds__(64 * NW, NB == 8 || (NB == 4 && (NW == 8 || (KV == 
   }
   const int kv = it / hgs, hg = it % hgs;
   const int h0 = kv * G + hg * 16, nh = min(16, G - hg * 16);
-  // q on its way first (eight dims of each block, in their own order): it hangs on nothing
+  // q on its way first (eight dims of each block, in their own order): it hangs on nothing.
+  // (`out` may be q: a row's heads are written after the waves that read them have met, or by the join)
   f4u_t qx[NB][2];
   {
     const int64_t o = r * a.q_ld + (int64_t)(h0 + min(PACK ? col & 3 : col, nh - 1)) * HD + 8 * g;

@@ -90,10 +90,12 @@ class PagedKv(_native.Cache):
     attend(q, seqs, lengths, *, scale=head_dim ** -0.5, window=0, out=None) -> out
         Attention of rows q [n, heads, head_dim] over the first lengths[i] positions of
         sequence seqs[i] (the last `window` of them where given). Length 0 gives zeros.
+        `out` may be q.
 
     Rows are float32 or float16 and may be strided (a row's heads and dims together);
     seqs, positions and lengths are contiguous int32 [n]. Rows with a negative sequence
-    are left out: their results stay as they were. The operators have no gradient.
+    are left out: their results stay as they were (without `out`, as new memory is).
+    The operators have no gradient.
     """
 
     def __init__(self, pages: torch.Tensor, table: torch.Tensor, kv_heads: int, head_dim: int, kv_dtype: str = "q8",

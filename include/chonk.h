@@ -333,7 +333,7 @@ typedef struct {
   const int32_t* seq;       /* [n] */
   const int32_t* lengths;   /* [n] positions of the sequence that the row sees */
   const void* q;            /* [n][heads][head_dim] */
-  void* out;                /* [n][heads][head_dim] */
+  void* out;                /* [n][heads][head_dim]; may be q */
   int64_t q_stride, out_stride;
   float scale;
   int32_t window;           /* the last `window` of those positions alone; 0: all */

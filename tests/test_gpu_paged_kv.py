@@ -275,6 +275,22 @@ def test_sizes_of_values_and_half_precision_rows(kv):
                 assert np.all((np.abs(got - want) <= tol)[fine]), float((np.abs(got - want) / tol)[fine].max())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("max_pages", [3, 70])
+def test_attend_over_q_itself(dtype, max_pages):
+    """Results that take q's place, whole rows and cut ones, one left out."""
+    c = Cache("q8", 2, 64, n_seqs=3, max_pages=max_pages, seed=max_pages)
+    n = 40
+    q = dev(c.rng.standard_normal((n, 36, 64)), dtype)
+    seqs = c.rng.integers(0, 3, n).astype(np.int32)
+    seqs[5] = -1
+    lengths = dev(c.rng.integers(0, 64 * max_pages + 1, n).astype(np.int32))
+    apart = c.op.attend(q, dev(seqs), lengths, out=q.clone())
+    assert c.op.attend(q, dev(seqs), lengths, out=q) is q
+    c.op.check()
+    assert torch.equal(q, apart)
+
+
 @pytest.mark.parametrize("kv", ref.TYPES)
 @pytest.mark.parametrize("heads,kv_heads,hd", [(16, 1, 256), (9, 1, 256), (5, 1, 128), (8, 8, 32), (32, 2, 64)])
 @pytest.mark.parametrize("max_pages", [1, 70])
